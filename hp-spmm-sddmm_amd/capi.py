@@ -73,6 +73,10 @@ def flags_with_options(flags=0, **options):
     return FlagsWithOptions(flags, options)
 
 
+# hpspmm_dtype, hpspmm_id_type
+F32, BF16, F16 = 0, 1, 2
+I32, I64 = 0, 1
+
 STRATEGY_ROWS = 1
 STRATEGY_SEGMENTS = 2
 STRATEGY_GENERIC_K = 3
@@ -87,6 +91,8 @@ EXPORTS = (
     "hpspmm_fill_f32", "hpspmm_csr_spmm_timed", "hpspmm_plan_bind_values", "hpspmm_plan_create_ordered",
     "hpspmm_csr_spmm_static", "hpspmm_csr_spmm_timed_launches", "hpspmm_plan_create_ex",
     "hpspmm_static_workspace_init", "hpspmm_csr_spmm_timed_min", "hpspmm_get_device_info",
+    "hpspmm_rows_plan_create", "hpspmm_rows_plan_destroy", "hpspmm_embedding_lookup", "hpspmm_embedding_grad",
+    "hpspmm_group_rows", "hpspmm_grouped_mm", "hpspmm_grouped_mm_grad_x", "hpspmm_grouped_mm_grad_w",
 )
 
 _i64 = ctypes.c_int64
@@ -175,6 +181,15 @@ def lib():
         L.hpspmm_csr_spmm_timed_launches.argtypes = [_p, _p, _p, _p, _p, _p, _p, ctypes.c_int, ctypes.c_int,
                                                      ctypes.c_int, ctypes.POINTER(ctypes.c_float),
                                                      ctypes.POINTER(ctypes.c_char_p), ctypes.POINTER(ctypes.c_int)]
+        i, f = ctypes.c_int, ctypes.c_float
+        L.hpspmm_rows_plan_create.argtypes = [_i64, _i64, _i64, ctypes.POINTER(_p)]
+        L.hpspmm_rows_plan_destroy.argtypes = [_p]
+        L.hpspmm_embedding_lookup.argtypes = [_i64, _i64, _i64, _p, i, _p, _i64, i, f, _p, _i64, _p]
+        L.hpspmm_embedding_grad.argtypes = [_p, _i64, _i64, _i64, _p, i, _p, _i64, i, f, _p, _i64, i, i, _p]
+        L.hpspmm_group_rows.argtypes = [_p, _i64, _i64, _p, i, _p, _p, _p]
+        L.hpspmm_grouped_mm.argtypes = [_i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _i64, _p, _p, _i64, i, _p]
+        L.hpspmm_grouped_mm_grad_x.argtypes = L.hpspmm_grouped_mm.argtypes
+        L.hpspmm_grouped_mm_grad_w.argtypes = [_p, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _i64, i, i, i, _p]
         _lib = L
     return _lib
 
@@ -380,3 +395,177 @@ def csr_spmm_timed_launches(plan, rowptr, col, val, B, C, warmup=5, iters=50, st
     check(lib().hpspmm_csr_spmm_timed_launches(plan._h, _ptr(rowptr), _ptr(col), _ptr(val), _ptr(B), _ptr(C),
                                                _stream(stream), warmup, iters, cap, ms, names, ctypes.byref(n)))
     return [(names[i].decode(), float(ms[i])) for i in range(n.value)]
+
+
+# ---- row operators -------------------------------------------------------------------------------------------------
+
+_dtypes = None  # {torch type: hpspmm_dtype}, {torch type: hpspmm_id_type}
+
+
+def _types():
+    global _dtypes
+    if _dtypes is None:
+        import torch
+        _dtypes = ({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}, {torch.int32: I32, torch.int64: I64})
+    return _dtypes
+
+
+def _row_arg(t, name, device=None):
+    """A GPU tensor, on the same device as the operands before it."""
+    if not getattr(t, "is_cuda", False):
+        raise TypeError(f"{name} must be a torch tensor in GPU memory")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the other operands on {device}")
+    return t.device
+
+
+def _rows_matrix(t, name, shape, device, dtype=None):
+    """(address, leading dimension, hpspmm_dtype) of a matrix whose rows are contiguous."""
+    _row_arg(t, name, device)
+    kind = _types()[0].get(t.dtype)
+    if kind is None or (dtype is not None and t.dtype != dtype):
+        raise TypeError(f"{name} must be {dtype if dtype is not None else 'float32, bfloat16 or float16'}, got {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+    rows, width = shape[-2:]
+    ld = t.stride(-2) if rows > 1 else width
+    if (width > 1 and t.stride(-1) != 1) or ld < width:
+        raise ValueError(f"{name} must have contiguous rows that do not overlap, got strides {t.stride()}")
+    return t.data_ptr(), ld, kind
+
+
+def _row_ids(t, name, device=None):
+    d = _row_arg(t, name, device)
+    kind = _types()[1].get(t.dtype)
+    if kind is None or t.dim() != 1 or not t.is_contiguous():
+        raise TypeError(f"{name} must be a contiguous vector of int32 or int64")
+    return d, t.data_ptr(), kind
+
+
+def _offsets(t, name, entries, device):
+    import torch
+    _row_arg(t, name, device)
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+        raise TypeError(f"{name} must be a contiguous vector of int32")
+    if t.numel() != entries:
+        raise ValueError(f"{name} must have {entries} entries, got {t.numel()}")
+    return t.data_ptr()
+
+
+def _call_on(device, stream, function, *args):
+    """function(*args, stream) with `device` current, on `stream` or that device's current one."""
+    import torch
+    if torch.cuda.current_device() == device.index:
+        st = torch.cuda.current_stream() if stream is None else stream
+        return check(function(*args, st.cuda_stream))
+    with torch.cuda.device(device):
+        st = torch.cuda.current_stream() if stream is None else stream
+        return check(function(*args, st.cuda_stream))
+
+
+class RowsPlan:
+    """Owns an hpspmm_rows_plan: workspace for up to max_rows rows, ids below max_ids and rows of max_width columns
+    (see hpspmm_rows_plan_create in include/hpspmm.h), on `device` (default: the current one)."""
+
+    def __init__(self, max_rows, max_ids, max_width=0, device=None):
+        import torch
+        self._h = ctypes.c_void_p()
+        self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        with torch.cuda.device(self.device):
+            self.device = torch.device("cuda", torch.cuda.current_device())
+            check(lib().hpspmm_rows_plan_create(max_rows, max_ids, max_width, ctypes.byref(self._h)))
+
+    def destroy(self):
+        if getattr(self, "_h", None):
+            lib().hpspmm_rows_plan_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        # at interpreter exit the module's globals may already be gone; the process frees the plan
+        try:
+            self.destroy()
+        except Exception:
+            pass
+
+
+def _plan_handle(plan):
+    if not isinstance(plan, RowsPlan) or not plan._h:
+        raise TypeError("plan must be a RowsPlan that has not been destroyed")
+    return plan._h
+
+
+def embedding_lookup(table, ids, out, scale=1.0, stream=None):
+    """out[i] = scale * table[ids[i]] through hpspmm_embedding_lookup; zeros where ids[i] is outside the table."""
+    device, ids_p, id_kind = _row_ids(ids, "ids")
+    n, (vocab, width) = ids.shape[0], table.shape
+    table_p, ld_table, kind = _rows_matrix(table, "table", (vocab, width), device)
+    out_p, ld_out, _ = _rows_matrix(out, "out", (n, width), device, table.dtype)
+    _call_on(device, stream, lib().hpspmm_embedding_lookup, n, vocab, width, ids_p, id_kind, table_p, ld_table, kind,
+             scale, out_p, ld_out)
+    return out
+
+
+def embedding_grad(plan, ids, grad, d_table, scale=1.0, accumulate=False, stream=None):
+    """d_table[v] (+)= scale * the sum of grad[i] over ids[i] == v through hpspmm_embedding_grad."""
+    handle = _plan_handle(plan)
+    device, ids_p, id_kind = _row_ids(ids, "ids", plan.device)
+    n, (vocab, width) = ids.shape[0], d_table.shape
+    grad_p, ld_grad, grad_kind = _rows_matrix(grad, "grad", (n, width), device)
+    table_p, ld_table, table_kind = _rows_matrix(d_table, "d_table", (vocab, width), device)
+    _call_on(device, stream, lib().hpspmm_embedding_grad, handle, n, vocab, width, ids_p, id_kind, grad_p,
+             ld_grad, grad_kind, scale, table_p, ld_table, table_kind, bool(accumulate))
+    return d_table
+
+
+def group_rows(plan, ids, groups, order, offsets, stream=None):
+    """(order, offsets): the rows sorted by id and where every group begins, through hpspmm_group_rows."""
+    handle = _plan_handle(plan)
+    device, ids_p, id_kind = _row_ids(ids, "ids", plan.device)
+    n = ids.shape[0]
+    order_p = _offsets(order, "order", n, device)
+    offsets_p = _offsets(offsets, "offsets", groups + 1, device)
+    _call_on(device, stream, lib().hpspmm_group_rows, handle, n, groups, ids_p, id_kind, order_p, offsets_p)
+    return order, offsets
+
+
+def _weights(t, name, shape, device, dtype):
+    address, ld, kind = _rows_matrix(t, name, shape, device, dtype)
+    return address, ld, (t.stride(0) if shape[0] > 1 else 0), kind
+
+
+def grouped_mm(x, w, offsets, y, stream=None):
+    """y[i] = x[i] @ w[e].T for the rows i of every group e through hpspmm_grouped_mm."""
+    device = _row_arg(x, "x")
+    (rows, k), (groups, m) = x.shape, w.shape[:2]
+    x_p, ld_x, kind = _rows_matrix(x, "x", (rows, k), device)
+    w_p, ld_w, stride_w, _ = _weights(w, "w", (groups, m, k), device, x.dtype)
+    y_p, ld_y, _ = _rows_matrix(y, "y", (rows, m), device, x.dtype)
+    _call_on(device, stream, lib().hpspmm_grouped_mm, rows, groups, k, m, x_p, ld_x, w_p, ld_w, stride_w,
+             _offsets(offsets, "offsets", groups + 1, device), y_p, ld_y, kind)
+    return y
+
+
+def grouped_mm_grad_x(dy, w, offsets, dx, stream=None):
+    """dx[i] = dy[i] @ w[e] for the rows i of every group e through hpspmm_grouped_mm_grad_x."""
+    device = _row_arg(dy, "dy")
+    (rows, m), (groups, _, k) = dy.shape, w.shape
+    dy_p, ld_dy, kind = _rows_matrix(dy, "dy", (rows, m), device)
+    w_p, ld_w, stride_w, _ = _weights(w, "w", (groups, m, k), device, dy.dtype)
+    dx_p, ld_dx, _ = _rows_matrix(dx, "dx", (rows, k), device, dy.dtype)
+    _call_on(device, stream, lib().hpspmm_grouped_mm_grad_x, rows, groups, k, m, dy_p, ld_dy, w_p, ld_w, stride_w,
+             _offsets(offsets, "offsets", groups + 1, device), dx_p, ld_dx, kind)
+    return dx
+
+
+def grouped_mm_grad_w(plan, dy, x, offsets, dw, accumulate=False, stream=None):
+    """dw[e] (+)= the sum of dy[i].T @ x[i] over the rows i of group e through hpspmm_grouped_mm_grad_w."""
+    handle = _plan_handle(plan)
+    device = _row_arg(dy, "dy", plan.device)
+    (rows, m), k, groups = dy.shape, x.shape[1], dw.shape[0]
+    dy_p, ld_dy, kind = _rows_matrix(dy, "dy", (rows, m), device)
+    x_p, ld_x, _ = _rows_matrix(x, "x", (rows, k), device, dy.dtype)
+    dw_p, ld_dw, stride_dw, dw_kind = _weights(dw, "dw", (groups, m, k), device, None)
+    _call_on(device, stream, lib().hpspmm_grouped_mm_grad_w, handle, rows, groups, k, m, dy_p, ld_dy, x_p,
+             ld_x, _offsets(offsets, "offsets", groups + 1, device), dw_p, ld_dw, stride_dw, kind, dw_kind,
+             bool(accumulate))
+    return dw

@@ -413,6 +413,99 @@ int hpspmm_csr_spmm_timed_launches(hpspmm_plan *plan, const int32_t *d_rowptr, c
                                    int warmup, int iters, int max_launches, float *mean_ms_out,
                                    const char **names_out, int *n_launches_out);
 
+/*
+ * Row operators: products with a sparse factor that is given by one id per row
+ * instead of CSR arrays.  A lookup is A * table with one nonzero (scale) in
+ * every row of A; its gradient is A^T times the rows' gradients; a product
+ * grouped by expert is a product with a matrix of dense blocks, one per group
+ * of rows.  The reference has no counterpart.  They take matrices of 32- or
+ * 16-bit elements, row-major with any leading dimension >= the row length;
+ * every sum is held in 32 bits and rounded once, to nearest even.
+ *
+ *   - ids are int32 or int64; an id outside [0, ids) belongs to no row: its
+ *     place is padding, never an access out of range.
+ *   - Calls only launch kernels (no allocation, no memset, no host
+ *     synchronisation): they may be captured in a HIP graph, and a replay
+ *     reads ids, offsets and operands as they are then.  No result depends on
+ *     the order in which workgroups run: the same inputs give the same bits.
+ *   - Outputs must not overlap inputs.
+ *   - Addresses may be any multiple of the element size; rows at multiples of
+ *     16 bytes (addresses and leading dimensions) are read and written faster.
+ */
+typedef enum hpspmm_dtype { HPSPMM_F32 = 0, HPSPMM_BF16 = 1, HPSPMM_F16 = 2 } hpspmm_dtype;
+typedef enum hpspmm_id_type { HPSPMM_I32 = 0, HPSPMM_I64 = 1 } hpspmm_id_type;
+
+/*
+ * Workspace of the row operators that sort or split, made once for the largest
+ * sizes to come and kept: rows, ids (vocabulary or groups) and columns per row
+ * (0 where hpspmm_embedding_grad is not called).  It lives on the device that
+ * is current here and is used from one stream at a time; two captured graphs
+ * that use the same plan must not run at the same time.
+ */
+typedef struct hpspmm_rows_plan hpspmm_rows_plan;
+int hpspmm_rows_plan_create(int64_t max_rows, int64_t max_ids, int64_t max_width, hpspmm_rows_plan **plan_out);
+/* Frees the plan's device memory.  NULL is accepted. */
+int hpspmm_rows_plan_destroy(hpspmm_rows_plan *plan);
+
+/*
+ * out[i, :] = scale * table[ids[i], :] for i in [0, n); a row of zeros where
+ * ids[i] is outside [0, vocab).  table is vocab x width, out is n x width, both
+ * of type `dtype`; the product is formed in 32 bits.
+ */
+int hpspmm_embedding_lookup(int64_t n, int64_t vocab, int64_t width, const void *d_ids, int id_type,
+                            const void *d_table, int64_t ld_table, int dtype, float scale, void *d_out,
+                            int64_t ld_out, void *stream);
+
+/*
+ * The gradient of hpspmm_embedding_lookup:
+ *   table[v, :] = (accumulate ? table[v, :] : 0) + scale * sum of grad[i, :] over ids[i] = v
+ * grad is n x width of type grad_type, table vocab x width of type table_type
+ * (any pair of types).  Without `accumulate` every row of the table is written,
+ * zeros where no id points; with it the rows that no id points at are not
+ * touched.  The rows of one id are added in an order that depends on the ids
+ * alone.
+ */
+int hpspmm_embedding_grad(hpspmm_rows_plan *plan, int64_t n, int64_t vocab, int64_t width, const void *d_ids,
+                          int id_type, const void *d_grad, int64_t ld_grad, int grad_type, float scale, void *d_table,
+                          int64_t ld_table, int table_type, int accumulate, void *stream);
+
+/*
+ * order[0..n) = the rows sorted by id, rows of one id in increasing order,
+ * padding last; offsets[g] = number of rows whose id is in [0, g), for g =
+ * 0..groups.  The rows of group g are order[offsets[g] .. offsets[g + 1]).
+ */
+int hpspmm_group_rows(hpspmm_rows_plan *plan, int64_t n, int64_t groups, const void *d_ids, int id_type,
+                      int32_t *d_order, int32_t *d_offsets, void *stream);
+
+/*
+ * Products grouped by expert: rows offsets[e] .. offsets[e + 1] - 1 of x belong
+ * to group e and meet its m x k matrix w[e] (rows ld_w elements apart, matrices
+ * stride_w elements apart).  offsets holds groups + 1 entries on the device,
+ * not decreasing, within [0, rows]; rows of no group are not read and stay as
+ * they are in the output.  (Offsets that are otherwise give unspecified values,
+ * never an access out of range.)  groups <= 65535; k, m <= 2^20.
+ *
+ *   hpspmm_grouped_mm           y[i, :]  = x[i, :] * w[e]^T     y is rows x m
+ *   hpspmm_grouped_mm_grad_x    dx[i, :] = dy[i, :] * w[e]      dx is rows x k
+ *   hpspmm_grouped_mm_grad_w    dw[e] = (accumulate ? dw[e] : 0) + sum of dy[i, :]^T * x[i, :]
+ *
+ * Operands are of one type; dw is of that type or HPSPMM_F32.  A group without
+ * rows gets a dw of zeros (or keeps its own with `accumulate`).  Weights that
+ * are stored k x m go through hpspmm_grouped_mm_grad_x for the product and
+ * hpspmm_grouped_mm for its gradient, with k and m exchanged.  The plan may be
+ * of any size (hpspmm_grouped_mm_grad_w splits long sums through it).
+ */
+int hpspmm_grouped_mm(int64_t rows, int64_t groups, int64_t k, int64_t m, const void *d_x, int64_t ld_x,
+                      const void *d_w, int64_t ld_w, int64_t stride_w, const int32_t *d_offsets, void *d_y,
+                      int64_t ld_y, int dtype, void *stream);
+int hpspmm_grouped_mm_grad_x(int64_t rows, int64_t groups, int64_t k, int64_t m, const void *d_dy, int64_t ld_dy,
+                             const void *d_w, int64_t ld_w, int64_t stride_w, const int32_t *d_offsets, void *d_dx,
+                             int64_t ld_dx, int dtype, void *stream);
+int hpspmm_grouped_mm_grad_w(hpspmm_rows_plan *plan, int64_t rows, int64_t groups, int64_t k, int64_t m,
+                             const void *d_dy, int64_t ld_dy, const void *d_x, int64_t ld_x, const int32_t *d_offsets,
+                             void *d_dw, int64_t ld_dw, int64_t stride_dw, int dtype, int dw_type, int accumulate,
+                             void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,562 @@
+"""Row operators on the GPU, through the python entry points, against plain implementations in 64 bits.
+
+Tolerances follow from the arithmetic that the operators promise (sums in 32 bits, one rounding at the end), with
+u = eps / 2 of a type: a product or sum of L terms formed in 32 bits is off by at most (L + 2) * 2 * u32 * sum |terms|
+(2: a matrix instruction may cut where an addition rounds), its rounding to the output's type by u * |value|, or by half
+of that type's smallest step where values are below its normal range.
+"""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+KINDS = ["float32", "bfloat16", "float16"]
+
+
+def _torch():
+    import torch
+    return torch
+
+
+def _t(kind):
+    return getattr(_torch(), kind)
+
+
+def _bound(value, absolute, terms, dtype):
+    torch = _torch()
+    f = torch.finfo(dtype)
+    u32 = torch.finfo(torch.float32).eps / 2
+    sums = (terms + 2) * 2 * u32 * absolute
+    return sums + (value.abs() + sums) * (f.eps / 2) + f.smallest_normal * f.eps / 2
+
+
+def _check(got, value, absolute, terms, what=""):
+    assert got.shape == value.shape
+    off = (got.double() - value).abs() - _bound(value, absolute, terms, got.dtype)
+    assert not torch_isnan(got), what
+    worst = off.max().item() if off.numel() else -1.0
+    assert worst <= 0, f"{what}: {worst:.3g} beyond the bound at {np.unravel_index(int(off.argmax()), tuple(off.shape))}"
+
+
+def torch_isnan(x):
+    return bool(_torch().isnan(x).any())
+
+
+def _gen(gpu, seed):
+    return _torch().Generator(device=gpu).manual_seed(seed)
+
+
+def _matrix(gpu, g, rows, width, kind, layout):
+    """A matrix of normal values, contiguous or inside a wider one; what surrounds it is NaN: reading it would show."""
+    torch = _torch()
+    if layout == "contiguous":
+        return torch.randn(rows, width, device=gpu, generator=g).to(_t(kind))
+    before, after = (8, 24) if layout == "aligned_slice" else (1, 2)
+    big = torch.full((rows + 2, before + width + after), float("nan"), device=gpu, dtype=_t(kind))
+    view = big[1:rows + 1, before:before + width]
+    view.copy_(torch.randn(rows, width, device=gpu, generator=g))
+    return view
+
+
+class Guarded:
+    """An output inside a wider buffer of a known value: what lies around it must not change."""
+
+    def __init__(self, gpu, shape, kind, layout, fill=float("nan")):
+        torch = _torch()
+        before, after = {"contiguous": (0, 0), "aligned_slice": (16, 8), "odd_slice": (3, 2)}[layout]
+        *lead, rows, width = shape
+        self.big = torch.full((*lead, rows + 2, before + width + after), 77.0, device=gpu, dtype=_t(kind))
+        self.view = self.big[..., 1:rows + 1, before:before + width]
+        self.view.fill_(fill)
+        self.fill = fill
+
+    def check_around(self):
+        rest = self.big.clone()
+        torch = _torch()
+        view = torch.as_strided(rest, self.view.shape, self.view.stride(), self.view.storage_offset())
+        view.fill_(77.0)
+        assert bool((rest == 77.0).all()), "something beside the output was written"
+
+
+def _ids(gpu, g, n, ids, kind, how="mixed"):
+    torch = _torch()
+    if how == "one":
+        t = torch.full((n,), ids // 2, device=gpu)
+    elif how == "none":
+        t = torch.where(torch.rand(n, device=gpu, generator=g) < 0.5, -1, ids)
+    else:
+        # a few ids are frequent; padding and ids beyond the table in between
+        u = torch.rand(n, device=gpu, generator=g, dtype=torch.float64)
+        t = (ids * u ** 4).long().clamp(max=ids - 1)
+        r = torch.rand(n, device=gpu, generator=g)
+        t[r < 0.1] = -1
+        t[r > 0.95] = ids
+        if kind == "int64":
+            t[(r > 0.93) & (r < 0.95)] = (1 << 32) + 1  # its low 32 bits alone would be an id
+    return t.to(_t(kind))
+
+
+def _in_table(ids, vocab):
+    t = ids.long()
+    return (t >= 0) & (t < vocab)
+
+
+# ---- lookup ---------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("id_kind", ["int32", "int64"])
+@pytest.mark.parametrize("layout", ["contiguous", "aligned_slice", "odd_slice"])
+@pytest.mark.parametrize("n, vocab, width", [(1, 1, 1), (3, 5, 7), (17, 100, 64), (1000, 331, 129), (257, 50, 2056),
+                                             (40000, 1000, 40), (9000, 70, 1024)])
+def test_lookup(pkg, gpu, kind, id_kind, layout, n, vocab, width):
+    torch = _torch()
+    g = _gen(gpu, n + width)
+    table = _matrix(gpu, g, vocab, width, kind, layout)
+    ids = _ids(gpu, g, n, vocab, id_kind)
+    out = Guarded(gpu, (n, width), kind, layout)
+    scale = 5.65685424949
+    assert pkg.capi.embedding_lookup(table, ids, out.view, scale=scale) is out.view
+    here = _in_table(ids, vocab)
+    want = table[torch.where(here, ids.long(), 0)].double() * float(np.float32(scale))
+    # one product in 32 bits and one rounding
+    f = torch.finfo(out.view.dtype)
+    tol = want.abs() * (f.eps / 2 + 2.0 ** -24) * (1 + 2.0 ** -8) + f.smallest_normal * f.eps / 2
+    got = out.view.double()
+    assert bool(((got - want).abs() <= tol)[here].all())
+    assert not got[~here].any() and not torch_isnan(got)
+    out.check_around()
+
+
+def test_lookup_in_an_empty_table(pkg, gpu):
+    torch = _torch()
+    out = torch.full((5, 24), 3.0, device=gpu)
+    pkg.capi.embedding_lookup(torch.empty(0, 24, device=gpu), torch.arange(5, device=gpu), out)
+    assert not out.any()
+
+
+def test_lookup_beyond_32_bit_offsets(pkg, gpu):
+    """A table and an output of more than 2^32 bytes and 2^31 elements, the rows met at their far ends."""
+    torch = _torch()
+    vocab, width = (1 << 19) + 3, 4104
+    table = torch.zeros(vocab, width, device=gpu, dtype=torch.bfloat16)
+    far = torch.tensor([0, 1, vocab - 2, vocab - 1], device=gpu)
+    table[far] = torch.randn(4, width, device=gpu).to(torch.bfloat16)
+    ids = far.repeat(-(-vocab // 4))[:vocab].contiguous()
+    out = torch.empty(vocab, width, device=gpu, dtype=torch.bfloat16)
+    pkg.capi.embedding_lookup(table, ids, out)
+    for rows in (slice(0, 9), slice(vocab - 9, vocab)):
+        assert torch.equal(out[rows], table[ids[rows]])
+
+
+# ---- gradient of the lookup -----------------------------------------------------------------------------------------
+
+def _grad_reference(ids, grad, vocab, scale):
+    torch = _torch()
+    here = _in_table(ids, vocab)
+    at, x = ids.long()[here], grad[here].double() * float(np.float32(scale))
+    value = torch.zeros(vocab, grad.shape[1], device=grad.device, dtype=torch.float64).index_add_(0, at, x)
+    absolute = torch.zeros_like(value).index_add_(0, at, x.abs())
+    count = torch.zeros(vocab, 1, device=grad.device, dtype=torch.float64).index_add_(
+        0, at, torch.ones(at.shape[0], 1, device=grad.device, dtype=torch.float64))
+    return value, absolute, count
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("out_kind", ["same", "float32"])
+@pytest.mark.parametrize("layout", ["contiguous", "aligned_slice", "odd_slice"])
+@pytest.mark.parametrize("how", ["mixed", "one", "none"])
+@pytest.mark.parametrize("n, vocab, width", [(1, 1, 1), (7, 3, 5), (100, 1000, 64), (3001, 257, 129), (9000, 40, 520),
+                                             (40000, 70000, 24)])
+def test_lookup_gradient(pkg, gpu, kind, out_kind, layout, how, n, vocab, width):
+    g = _gen(gpu, n + vocab)
+    out_kind = kind if out_kind == "same" else out_kind
+    ids = _ids(gpu, g, n, vocab, "int64" if layout == "contiguous" else "int32", how)
+    grad = _matrix(gpu, g, n, width, kind, layout)
+    plan = pkg.capi.RowsPlan(n, vocab, width)
+    out = Guarded(gpu, (vocab, width), out_kind, layout)
+    assert pkg.capi.embedding_grad(plan, ids, grad, out.view, scale=0.75) is out.view
+    value, absolute, count = _grad_reference(ids, grad, vocab, 0.75)
+    _check(out.view, value, absolute, count, "sum")
+    assert not out.view[count[:, 0] == 0].any()
+    out.check_around()
+    # added onto what is there; rows that no id points at stay bit for bit (a NaN among them)
+    base = Guarded(gpu, (vocab, width), out_kind, layout)
+    torch = _torch()
+    base.view.copy_(torch.randn(vocab, width, device=gpu, generator=g))
+    base.view[count[:, 0] == 0] = float("nan")
+    before = base.view.clone()
+    pkg.capi.embedding_grad(plan, ids, grad, base.view, scale=0.75, accumulate=True)
+    met = count[:, 0] > 0
+    old = before.double()
+    _check(base.view[met], (value + old)[met], (absolute + old.abs())[met], (count + 1)[met], "accumulated")
+    assert bool(torch.isnan(base.view[~met]).all())
+    base.check_around()
+    plan.destroy()
+
+
+def test_lookup_gradient_against_differences(pkg, gpu):
+    """The gradient of L = sum(c * lookup(table)) in the direction d, against (L(table + h d) - L(table - h d)) / 2h:
+    the lookup is linear, so the difference is exact up to rounding (values are small whole numbers: no rounding at all)."""
+    torch = _torch()
+    g = _gen(gpu, 3)
+    n, vocab, width = 500, 60, 40
+    whole = lambda *s: torch.randint(-4, 5, s, device=gpu, generator=g).float()  # noqa: E731
+    table, d, c = whole(vocab, width), whole(vocab, width), whole(n, width)
+    ids = _ids(gpu, g, n, vocab, "int32")
+
+    def loss(t):
+        out = torch.empty(n, width, device=gpu)
+        return (pkg.capi.embedding_lookup(t, ids, out, scale=2.0) * c).sum().item()
+
+    plan = pkg.capi.RowsPlan(n, vocab, width)
+    grad = torch.empty(vocab, width, device=gpu)
+    pkg.capi.embedding_grad(plan, ids, c, grad, scale=2.0)
+    assert (loss(table + d) - loss(table - d)) / 2 == (grad * d).sum().item()
+
+
+def test_lookup_gradient_is_reproducible(pkg, gpu):
+    torch = _torch()
+    g = _gen(gpu, 5)
+    n, vocab, width = 30000, 500, 200
+    ids, grad = _ids(gpu, g, n, vocab, "int64"), torch.randn(n, width, device=gpu, generator=g)
+    got = []
+    for _ in range(3):
+        plan = pkg.capi.RowsPlan(n + 1000 * len(got), vocab, width + 8 * len(got))
+        got.append(pkg.capi.embedding_grad(plan, ids, grad, torch.empty(vocab, width, device=gpu)))
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+
+
+def test_plan_limits_are_kept(pkg, gpu):
+    torch = _torch()
+    capi = pkg.capi
+    plan = capi.RowsPlan(100, 50, 32)
+    ids = torch.zeros(100, dtype=torch.int64, device=gpu)
+    grad = lambda n, w: torch.zeros(n, w, device=gpu)  # noqa: E731
+    capi.embedding_grad(plan, ids, grad(100, 32), grad(50, 32))
+    for n, vocab, width in ((101, 50, 32), (100, 51, 32), (100, 50, 33)):
+        with pytest.raises(capi.HpSpmmError, match="the plan is for"):
+            capi.embedding_grad(plan, torch.zeros(n, dtype=torch.int64, device=gpu), grad(n, width), grad(vocab, width))
+    plan.destroy()
+    with pytest.raises(TypeError, match="destroyed"):
+        capi.embedding_grad(plan, ids, grad(100, 32), grad(50, 32))
+
+
+# ---- rows sorted by id ----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("id_kind", ["int32", "int64"])
+@pytest.mark.parametrize("how", ["mixed", "one", "none"])
+@pytest.mark.parametrize("n, groups", [(0, 4), (1, 1), (5, 300), (64, 8), (1000, 7), (2048, 64), (2049, 1000), (8192, 16),
+                                       (8193, 5000), (40000, 255), (70000, 256), (70000, 257), (300001, 130), (5000, 1 << 20)])
+def test_group_rows(pkg, gpu, id_kind, how, n, groups):
+    torch = _torch()
+    ids = _ids(gpu, _gen(gpu, n), n, groups, id_kind, how)
+    plan = pkg.capi.RowsPlan(n, groups)
+    order = torch.full((n + 2,), -7, device=gpu, dtype=torch.int32)
+    offsets = torch.full((groups + 3,), -7, device=gpu, dtype=torch.int32)
+    pkg.capi.group_rows(plan, ids, groups, order[1:n + 1], offsets[1:groups + 2])
+    key = torch.where(_in_table(ids, groups), ids.long(), groups)
+    want = torch.sort(key, stable=True).indices.to(torch.int32)
+    assert torch.equal(order[1:n + 1], want)
+    count = torch.bincount(key, minlength=groups + 1)[:groups]
+    assert torch.equal(offsets[2:groups + 2].long(), torch.cumsum(count, 0)) and offsets[1] == 0
+    assert order[0] == -7 and order[-1] == -7 and offsets[0] == -7 and offsets[-1] == -7
+
+
+# ---- products grouped by expert -------------------------------------------------------------------------------------
+
+def _offsets(rows, groups, how, seed):
+    """groups + 1 offsets; what is left of the rows belongs to no group."""
+    rng = np.random.default_rng(seed)
+    if how == "even":
+        sizes = [rows // groups] * groups
+        return np.concatenate([[0], np.cumsum(sizes)])
+    if how == "one":
+        sizes = [0] * groups
+        sizes[groups // 2] = rows
+        return np.concatenate([[0], np.cumsum(sizes)])
+    if how == "empty":
+        return np.zeros(groups + 1, dtype=np.int64)
+    cuts = np.sort(rng.integers(rows // 10, rows - rows // 10 + 1, groups + 1))  # ragged, a gap before and behind
+    if groups > 2:
+        cuts[groups // 2] = cuts[groups // 2 - 1]  # a group without rows
+    return cuts
+
+
+def _experts(gpu, seed, rows, groups, k, m, kind, layout, how):
+    torch = _torch()
+    g = _gen(gpu, seed)
+    off = _offsets(rows, groups, how, seed)
+    x, dy = _matrix(gpu, g, rows, k, kind, layout), _matrix(gpu, g, rows, m, kind, layout)
+    w = torch.randn(groups, m, k, device=gpu, generator=g).to(_t(kind))
+    if layout != "contiguous":
+        big = torch.full((groups, m + 1, k + (8 if layout == "aligned_slice" else 3)), float("nan"), device=gpu, dtype=_t(kind))
+        big[:, 1:, :k] = w
+        w = big[:, 1:, :k]
+    # rows of no group: NaN that must not reach any result
+    free = torch.ones(rows, dtype=torch.bool, device=gpu)
+    free[int(off[0]):int(off[-1])] = False
+    x[free] = float("nan")
+    dy[free] = float("nan")
+    return x, dy, w, off, torch.from_numpy(off.astype(np.int32)).to(gpu), free
+
+
+GROUPED = [(1, 1, 1, 1), (5, 3, 7, 9), (64, 4, 64, 64), (130, 3, 72, 200), (300, 5, 129, 65), (1000, 7, 256, 384),
+           (77, 33, 136, 264), (700, 2, 520, 1000), (513, 4, 31, 30)]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("layout", ["contiguous", "aligned_slice", "odd_slice"])
+@pytest.mark.parametrize("how", ["ragged", "even", "one", "empty"])
+@pytest.mark.parametrize("rows, groups, k, m", GROUPED)
+def test_grouped_products(pkg, gpu, kind, layout, how, rows, groups, k, m):
+    torch = _torch()
+    capi = pkg.capi
+    x, dy, w, off, offsets, free = _experts(gpu, rows + k, rows, groups, k, m, kind, layout, how)
+    y, dx = Guarded(gpu, (rows, m), kind, layout, fill=5.0), Guarded(gpu, (rows, k), kind, layout, fill=5.0)
+    assert capi.grouped_mm(x, w, offsets, y.view) is y.view
+    assert capi.grouped_mm_grad_x(dy, w, offsets, dx.view) is dx.view
+    plan = capi.RowsPlan(rows, groups)
+    dw = {t: Guarded(gpu, (groups, m, k), t, layout) for t in {kind, "float32"}}
+    for one in dw.values():
+        assert capi.grouped_mm_grad_w(plan, dy, x, offsets, one.view) is one.view
+    added = Guarded(gpu, (groups, m, k), "float32", layout)
+    start = torch.randn(groups, m, k, device=gpu, generator=_gen(gpu, 9))
+    added.view.copy_(start)
+    capi.grouped_mm_grad_w(plan, dy, x, offsets, added.view, accumulate=True)
+    for e in range(groups):
+        r = slice(int(off[e]), int(off[e + 1]))
+        n = r.stop - r.start
+        xe, de, we = x[r].double(), dy[r].double(), w[e].double()
+        _check(y.view[r], xe @ we.t().contiguous(), xe.abs() @ we.abs().t().contiguous(), k, f"y of group {e}")
+        _check(dx.view[r], de @ we, de.abs() @ we.abs(), m, f"dx of group {e}")
+        want, absolute = de.t().contiguous() @ xe, de.abs().t().contiguous() @ xe.abs()
+        for t, one in dw.items():
+            _check(one.view[e], want, absolute, n, f"dw of group {e} in {t}")
+        base = start[e].double()
+        _check(added.view[e], want + base, absolute + base.abs(), n + 1, f"dw of group {e} added")
+        if n == 0:
+            assert not dw[kind].view[e].any() and torch.equal(added.view[e], start[e])
+    assert bool((y.view[free] == 5.0).all()) and bool((dx.view[free] == 5.0).all()), "a row of no group was written"
+    for one in (y, dx, added, *dw.values()):
+        one.check_around()
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float32"])
+def test_grouped_products_with_offsets_that_are_none(pkg, gpu, kind):
+    """Offsets that decrease, are negative or lie beyond the rows: unspecified values, but nothing around is touched."""
+    torch = _torch()
+    capi = pkg.capi
+    rows, groups, k, m = 200, 5, 72, 136
+    x, dy, w, _, _, _ = _experts(gpu, 1, rows, groups, k, m, kind, "aligned_slice", "even")
+    plan = capi.RowsPlan(rows, groups)
+    for bad in ([0, 150, 30, 180, 60, 200], [-5, 10, 20, 30, 1000, 2000], [0, 0, 2**31 - 1, -2**31, 7, 300],
+                [200, 160, 120, 80, 40, 0]):
+        offsets = torch.tensor(bad, dtype=torch.int32, device=gpu)
+        outs = [Guarded(gpu, s, kind, "odd_slice") for s in ((rows, m), (rows, k), (groups, m, k))]
+        capi.grouped_mm(x, w, offsets, outs[0].view)
+        capi.grouped_mm_grad_x(dy, w, offsets, outs[1].view)
+        capi.grouped_mm_grad_w(plan, dy, x, offsets, outs[2].view)
+        torch.cuda.synchronize()
+        for one in outs:
+            one.check_around()
+
+
+def test_grouped_product_of_shared_weights(pkg, gpu):
+    """One matrix for all groups: a stride of zero between them."""
+    torch = _torch()
+    g = _gen(gpu, 2)
+    x = torch.randn(300, 64, device=gpu, generator=g).bfloat16()
+    w = torch.randn(1, 96, 64, device=gpu, generator=g).bfloat16().expand(4, -1, -1)
+    offsets = torch.tensor([0, 100, 100, 250, 300], dtype=torch.int32, device=gpu)
+    y = pkg.capi.grouped_mm(x, w, offsets, torch.empty(300, 96, device=gpu, dtype=torch.bfloat16))
+    a, b = x.double(), w[0].double()
+    _check(y, a @ b.t().contiguous(), a.abs() @ b.abs().t().contiguous(), 64)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_grouped_products_keep_nan_and_inf_in_their_rows(pkg, gpu, kind):
+    torch = _torch()
+    g = _gen(gpu, 4)
+    x = torch.randn(96, 80, device=gpu, generator=g).to(_t(kind))
+    w = torch.randn(3, 88, 80, device=gpu, generator=g).to(_t(kind))
+    x[7, 3], x[40, 79] = float("nan"), float("inf")
+    offsets = torch.tensor([0, 20, 50, 96], dtype=torch.int32, device=gpu)
+    y = pkg.capi.grouped_mm(x, w, offsets, torch.empty(96, 88, device=gpu, dtype=_t(kind)))
+    odd = ~torch.isfinite(y)
+    assert bool(odd[7].all()) and bool(odd[40].all())
+    odd[7], odd[40] = False, False
+    assert not odd.any()
+
+
+def test_grouped_gradients_against_differences(pkg, gpu):
+    """The gradients of L = sum(c * y) in the directions of x and w against central differences: whole numbers, exact."""
+    torch = _torch()
+    capi = pkg.capi
+    g = _gen(gpu, 6)
+    rows, groups, k, m = 90, 3, 40, 24
+    whole = lambda *s: torch.randint(-2, 3, s, device=gpu, generator=g).float()  # noqa: E731
+    x, w, c, du, dv = whole(rows, k), whole(groups, m, k), whole(rows, m), whole(rows, k), whole(groups, m, k)
+    offsets = torch.tensor([0, 31, 31, 90], dtype=torch.int32, device=gpu)
+
+    def loss(x, w):
+        return (capi.grouped_mm(x, w, offsets, torch.zeros(rows, m, device=gpu)) * c).double().sum().item()
+
+    dx = capi.grouped_mm_grad_x(c, w, offsets, torch.empty(rows, k, device=gpu))
+    dw = capi.grouped_mm_grad_w(capi.RowsPlan(0, 0), c, x, offsets, torch.empty(groups, m, k, device=gpu))
+    assert (loss(x + du, w) - loss(x - du, w)) / 2 == (dx * du).double().sum().item()
+    assert (loss(x, w + dv) - loss(x, w - dv)) / 2 == (dw * dv).double().sum().item()
+
+
+# ---- together -------------------------------------------------------------------------------------------------------
+
+def _routed_layer(capi, s):
+    """Tokens -> rows of a table -> one expert for each of two copies of every row -> their sum: forward and backward."""
+    capi.embedding_lookup(s["table"], s["tokens"], s["h"], scale=2.0)
+    capi.group_rows(s["plan"], s["expert"], s["groups"], s["order"], s["offsets"])
+    s["torch"].div(s["order"], 2, rounding_mode="floor", out=s["source"])  # row of every sorted copy
+    capi.embedding_lookup(s["h"], s["source"], s["x"])
+    capi.grouped_mm(s["x"], s["w"], s["offsets"], s["y"])
+    capi.embedding_grad(s["plan"], s["source"], s["y"], s["out"])
+    # backward: the gradient of every copy's output is its row's
+    capi.embedding_lookup(s["d_out"], s["source"], s["dy"])
+    capi.grouped_mm_grad_x(s["dy"], s["w"], s["offsets"], s["dx"])
+    capi.grouped_mm_grad_w(s["plan"], s["dy"], s["x"], s["offsets"], s["dw"])
+    capi.embedding_grad(s["plan"], s["source"], s["dx"], s["dh"])
+    capi.embedding_grad(s["plan"], s["tokens"], s["dh"], s["d_table"], scale=2.0)
+
+
+def _routed_state(pkg, gpu, kind, n=333, vocab=101, k=72, m=48, groups=5, seed=8):
+    torch = _torch()
+    g = _gen(gpu, seed)
+    r = lambda *s: torch.randn(*s, device=gpu, generator=g).to(_t(kind))  # noqa: E731
+    z = lambda *s: torch.zeros(*s, device=gpu, dtype=_t(kind))  # noqa: E731
+    i = lambda *s: torch.zeros(*s, device=gpu, dtype=torch.int32)  # noqa: E731
+    return {"torch": torch, "plan": pkg.capi.RowsPlan(2 * n, max(vocab, n, groups), max(k, m)), "groups": groups,
+            "tokens": _ids(gpu, g, n, vocab, "int64"), "expert": torch.randint(0, groups, (2 * n,), device=gpu, generator=g),
+            "table": r(vocab, k), "w": r(groups, m, k), "d_out": r(n, m), "h": z(n, k), "order": i(2 * n),
+            "offsets": i(groups + 1), "source": i(2 * n), "x": z(2 * n, k), "y": z(2 * n, m), "out": z(n, m),
+            "dy": z(2 * n, m), "dx": z(2 * n, k), "dh": z(n, k), "dw": torch.zeros(groups, m, k, device=gpu),
+            "d_table": torch.zeros(vocab, k, device=gpu)}
+
+
+def _routed_reference(s):
+    """The same in 64 bits, expert by expert from the ids themselves: (out, dw, d_table)."""
+    torch = s["torch"]
+    table, w, d_out = (s[q].double() for q in ("table", "w", "d_out"))
+    here = _in_table(s["tokens"], table.shape[0])
+    at = torch.where(here, s["tokens"].long(), 0)
+    h = torch.where(here[:, None], table[at] * 2.0, 0.0)
+    expert = s["expert"].view(-1, 2).long()
+    out, dh, dw = torch.zeros_like(d_out), torch.zeros_like(h), torch.zeros_like(w)
+    for e in range(w.shape[0]):
+        for c in range(2):
+            mine = (expert[:, c] == e).double()[:, None]
+            out += mine * (h @ w[e].t().contiguous())
+            dh += mine * (d_out @ w[e])
+            dw[e] += (mine * d_out).t().contiguous() @ h
+    d_table = torch.zeros_like(table).index_add_(0, at, torch.where(here[:, None], dh * 2.0, 0.0))
+    return out, dw, d_table
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_routed_layer(pkg, gpu, kind):
+    """All operators one after the other.  Every stage is within the rounding of its type of the exact one, so the last is
+    within the number of stages (5 of them round) times u, times the growth of a sum of k terms against its norm, which a
+    comparison in norms does not have: 8 u in all."""
+    torch = _torch()
+    s = _routed_state(pkg, gpu, kind)
+    _routed_layer(pkg.capi, s)
+    u = max(torch.finfo(_t(kind)).eps / 2, 2.0 ** -20)  # (sums of up to 700 terms in 32 bits)
+    for got, want in zip((s["out"], s["dw"], s["d_table"]), _routed_reference(s)):
+        rel = ((got.double() - want).norm() / want.norm()).item()
+        assert rel <= 8 * u, rel
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float32"])
+def test_captured_and_replayed(pkg, gpu, kind):
+    """The same run captured in a graph and replayed with other inputs, eager work and waits in between: the same bits."""
+    torch = _torch()
+    s = _routed_state(pkg, gpu, kind)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _routed_layer(pkg.capi, s)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _routed_layer(pkg.capi, s)
+    for seed in range(20, 25):
+        fresh = _routed_state(pkg, gpu, kind, seed=seed)
+        _routed_layer(pkg.capi, fresh)  # eager, with a plan and buffers of its own
+        for q in ("tokens", "expert", "table", "w", "d_out"):
+            s[q].copy_(fresh[q])
+        graph.replay()
+        torch.cuda.synchronize()
+        for q in ("out", "dw", "d_table", "order", "offsets"):
+            assert torch.equal(s[q], fresh[q]), (seed, q)
+
+
+def test_two_streams(pkg, gpu):
+    """Two plans on two streams at once, and a call on a stream that is not the current one."""
+    torch = _torch()
+    states = [_routed_state(pkg, gpu, "bfloat16", n=2000, seed=30 + i) for i in range(2)]
+    wants = []
+    for s in states:
+        _routed_layer(pkg.capi, s)
+        wants.append({q: s[q].clone() for q in ("out", "dw", "d_table")})
+        for q in ("out", "dw", "d_table"):
+            s[q].zero_()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in states]
+    for _ in range(5):
+        for s, st in zip(states, streams):
+            with torch.cuda.stream(st):
+                _routed_layer(pkg.capi, s)
+    torch.cuda.synchronize()
+    for s, want in zip(states, wants):
+        for q, v in want.items():
+            assert torch.equal(s[q], v), q
+    s = states[0]
+    s["h"].zero_()
+    torch.cuda.synchronize()
+    pkg.capi.embedding_lookup(s["table"], s["tokens"], s["h"], scale=2.0, stream=streams[1])
+    streams[1].synchronize()
+    assert s["h"].any()
+
+
+def test_operands_that_do_not_fit_are_refused(pkg, gpu):
+    torch = _torch()
+    capi = pkg.capi
+    f = lambda *s, t=torch.float32: torch.zeros(*s, device=gpu, dtype=t)  # noqa: E731
+    ids, off, plan = f(6, t=torch.int64), f(3, t=torch.int32), capi.RowsPlan(10, 10, 10)
+    bad = [
+        (ValueError, lambda: capi.embedding_lookup(f(9, 8), ids, f(5, 8))),
+        (ValueError, lambda: capi.embedding_lookup(f(9, 8), ids, f(6, 7))),
+        (TypeError, lambda: capi.embedding_lookup(f(9, 8), ids, f(6, 8, t=torch.float16))),
+        (TypeError, lambda: capi.embedding_lookup(f(9, 8, t=torch.float64), ids, f(6, 8, t=torch.float64))),
+        (TypeError, lambda: capi.embedding_lookup(f(9, 8), ids.float(), f(6, 8))),
+        (TypeError, lambda: capi.embedding_lookup(f(9, 8), f(6, 2, t=torch.int64)[:, 0], f(6, 8))),
+        (ValueError, lambda: capi.embedding_lookup(f(8, 9).t(), ids, f(6, 8))),
+        (ValueError, lambda: capi.embedding_lookup(f(9, 8), ids, f(1, 8).expand(6, 8))),
+        (TypeError, lambda: capi.embedding_lookup(f(9, 8).cpu(), ids, f(6, 8))),
+        (ValueError, lambda: capi.group_rows(plan, ids, 4, f(5, t=torch.int32), f(5, t=torch.int32))),
+        (ValueError, lambda: capi.group_rows(plan, ids, 4, f(6, t=torch.int32), f(4, t=torch.int32))),
+        (TypeError, lambda: capi.group_rows(plan, ids, 4, f(6, t=torch.int64), f(5, t=torch.int32))),
+        (ValueError, lambda: capi.grouped_mm(f(6, 8), f(2, 4, 7), off, f(6, 4))),
+        (ValueError, lambda: capi.grouped_mm(f(6, 8), f(2, 4, 8), off[:2], f(6, 4))),
+        (ValueError, lambda: capi.grouped_mm(f(6, 8), f(2, 4, 8), off, f(6, 5))),
+        (TypeError, lambda: capi.grouped_mm(f(6, 8), f(2, 4, 8, t=torch.float16), off, f(6, 4))),
+        (TypeError, lambda: capi.grouped_mm(f(6, 8), f(2, 4, 8), off.long(), f(6, 4))),
+        (ValueError, lambda: capi.grouped_mm_grad_x(f(6, 5), f(2, 4, 8), off, f(6, 8))),
+        (ValueError, lambda: capi.grouped_mm_grad_w(plan, f(6, 4), f(5, 8), off, f(2, 4, 8))),
+        (ValueError, lambda: capi.grouped_mm_grad_w(plan, f(6, 4), f(6, 8), off, f(2, 5, 8))),
+        (capi.HpSpmmError, lambda: capi.grouped_mm_grad_w(plan, f(6, 4), f(6, 8), off, f(2, 4, 8, t=torch.float16))),
+        (capi.HpSpmmError, lambda: capi.grouped_mm_grad_w(plan, f(6, 4), f(6, 8), off, f(1, 4, 8).expand(2, 4, 8))),
+        (TypeError, lambda: capi.grouped_mm_grad_w(None, f(6, 4), f(6, 8), off, f(2, 4, 8))),
+        (TypeError, lambda: capi.embedding_grad(None, ids, f(6, 8), f(9, 8))),
+    ]
+    for n, (error, call) in enumerate(bad):
+        with pytest.raises(error):
+            call()
+            pytest.fail(f"call {n} was not refused")
