@@ -1,7 +1,7 @@
 // Entry points of the products grouped by expert.
 #include "row_ops.hpp"
 
-#include "grouped_kernels.hpp"
+#include "grouped_tile_kernel.hpp"
 
 using namespace hpspmm_host;
 
@@ -35,23 +35,46 @@ int check_weights(const char* name, const void* p, int64_t groups, int64_t k, in
 // Row tiles of bm rows that the groups can have together, whatever their sizes.
 int64_t most_row_tiles(int64_t rows, int64_t groups, int64_t bm) { return std::min(rows, rows / bm + groups); }
 
+// Rows of an operand that 16-byte chunks cover whole, at multiples of 16 bytes, near enough together for 32-bit offsets
+// within a tile.
+bool chunked(const void* p, int64_t ld, int64_t stride, int64_t width, int64_t size) {
+  return aligned_to(p, 16) && ld * size % 16 == 0 && stride * size % 16 == 0 && width * size % 16 == 0 && ld < ((int64_t)1 << 21);
+}
+
+template <class T, class TO, int kMode, int kBM, int kBN, int kWM, int kWN, bool kDirect>
+int launch_tiles(const hpspmm::GroupedArgs& g, hipStream_t st) {
+  const int64_t n_out = kMode == hpspmm::kForward ? g.m : g.k;
+  const int64_t col_tiles = ceil_div(n_out, kBN);
+  const int64_t row_tiles = kMode == hpspmm::kGradW ? g.groups * ceil_div(g.m, kBM) : most_row_tiles(g.rows, g.groups, kBM);
+  const int64_t tiles = ceil_div(row_tiles * col_tiles, hpspmm::kXcds) * hpspmm::kXcds;
+  if (tiles == 0) return HPSPMM_OK;
+  if (tiles > INT32_MAX / (64 * kWM * kWN)) return fail(HPSPMM_ERR_INVALID_ARG, "the product has too many output tiles");
+  hipLaunchKernelGGL((hpspmm::grouped_tile_kernel<T, TO, kMode, kBM, kBN, kWM, kWN, kDirect>), dim3((unsigned)tiles),
+                     dim3(64 * kWM * kWN), 0, st, g, (int)col_tiles);
+  return HPSPMM_OK;
+}
+
 template <int kMode>
 int launch_grouped(const hpspmm::GroupedArgs& g, int dtype, int out_type, hipStream_t st) {
-  const int64_t n_out = kMode == hpspmm::kForward ? g.m : g.k;
-  const unsigned nt = (unsigned)ceil_div(n_out, hpspmm::kSimpleTile);
-  const dim3 grid = kMode == hpspmm::kGradW
-                        ? dim3((unsigned)ceil_div(g.m, hpspmm::kSimpleTile), nt, (unsigned)g.groups)
-                        : dim3((unsigned)most_row_tiles(g.rows, g.groups, hpspmm::kSimpleTile), nt, 1);
-  if (grid.x == 0 || grid.z == 0) return HPSPMM_OK;
-  dispatch_dtype(dtype, [&](auto t) {
+  const int64_t size = dtype_size(dtype);
+  const int64_t wide_a = kMode == hpspmm::kForward ? g.k : g.m;
+  const bool direct = chunked(g.a, g.lda, 0, wide_a, size) && chunked(g.b, g.ldb, g.stride_b, g.k, size);
+  int rc = dispatch_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     return dispatch_dtype(out_type, [&](auto o) {
       using TO = decltype(o);
-      if constexpr (std::is_same_v<T, TO> || (kMode == hpspmm::kGradW && std::is_same_v<TO, float>))
-        hipLaunchKernelGGL((hpspmm::grouped_simple_kernel<T, TO, kMode>), grid, dim3(hpspmm::kBlock), 0, st, g);
-      return HPSPMM_OK;
+      if constexpr (std::is_same_v<T, TO> || (kMode == hpspmm::kGradW && std::is_same_v<TO, float>)) {
+        if (!direct) return launch_tiles<T, TO, kMode, 128, 128, 2, 2, false>(g, st);
+        if constexpr (sizeof(T) == 2) {
+          if (g.rows >= 4096) return launch_tiles<T, TO, kMode, 256, 256, 2, 4, true>(g, st);
+        }
+        return launch_tiles<T, TO, kMode, 128, 128, 2, 2, true>(g, st);
+      } else {
+        return fail(HPSPMM_ERR_INVALID_ARG, "no product of these types");
+      }
     });
   });
+  if (rc) return rc;
   HPSPMM_HIP(hipGetLastError());
   return HPSPMM_OK;
 }

@@ -1,0 +1,306 @@
+// The tile kernel of the products grouped by expert: one workgroup per kBM x kBN tile of the output.
+//
+// Both operands of a step of the contraction (64 terms of 16-bit, 32 of 32-bit elements) lie in LDS in the layout they
+// have in memory, 16-byte chunks permuted within a row:
+//   row operand  kB rows of the tile, 128 bytes (8 chunks) of the contraction each      x, dy and w^T (forward)
+//   col operand  the step's rows, kB columns of the tile each                           w (gradient of x), dy and x (of w)
+// A fragment of a row operand is one 16-byte read a lane.  One of a col operand is read transposed: 16-bit elements with
+// the transposing 8-byte read (lane s of 16 gives the address of columns 4 (s % 4) ... + 3 of row s / 4 and receives
+// column s of the four rows), 32-bit ones word by word.  The permutations put what one read touches into different
+// banks: chunk c of row r lies at c ^ (r % 8) in a row operand; in a col operand the 32-byte (16-bit elements) or 64-byte
+// (32-bit) segments of the rows that a read meets are spread.
+//
+// Rows beyond the group and columns beyond the matrix repeat the last one that exists - what they give is not stored;
+// terms beyond the contraction are zeros in both operands, whatever lies there in memory.
+#pragma once
+
+#include "grouped_kernels.hpp"
+
+namespace hpspmm {
+
+typedef float float4_t __attribute__((ext_vector_type(4)));
+
+template <class T>
+struct Mfma;
+template <>
+struct Mfma<bf16_t> {
+  typedef bf16_t frag __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ float4_t mul(frag a, frag b, float4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mfma<f16_t> {
+  typedef f16_t frag __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ float4_t mul(frag a, frag b, float4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mfma<float> {
+  typedef float frag __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ float4_t mul(frag a, frag b, float4_t c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+  }
+};
+
+typedef __attribute__((address_space(3))) char lds_char;
+typedef __attribute__((address_space(3))) void lds_void;
+typedef short short4_t __attribute__((ext_vector_type(4)));
+
+// One operand of one output tile.
+template <class T, bool kCol, int kB, int kThreads, bool kDirect>
+struct Operand {
+  static constexpr int kSize = (int)sizeof(T);
+  static constexpr int kChunk = 16 / kSize;    // elements of a 16-byte chunk
+  static constexpr int kDepth = 8 * kChunk;    // terms of the contraction a step
+  static constexpr int kBytes = kB * 128;      // of LDS a step
+  static constexpr int kPer = kB * 8 / kThreads;  // chunks a thread brings in a step
+  static constexpr int kRowChunks = kCol ? kB / kChunk : 8;  // chunks of a row in LDS
+  static constexpr uint32_t kNowhere = 0xFFFFFFF0u;  // an offset beyond the buffer: the load gives zeros
+  using Chunk = typename Pack<T, kChunk, true>::type;
+
+  const char* base;    // first element of the step to be loaded
+  int64_t step;        // bytes from one step to the next
+  int64_t ld;          // bytes from row to row
+  int valid;           // rows (row operand) or columns (col operand) of the tile that exist
+  uint32_t offset[kDirect ? kPer : 1];
+
+  static __device__ __forceinline__ int swizzle(int r) {
+    if constexpr (!kCol) return r & 7;
+    else if constexpr (kSize == 2) return ((r & 3) | ((r >> 1) & 4)) << 1;
+    else return ((r >> 2) & 3) << 2;
+  }
+  // Row of LDS and chunk of that row in memory that this thread's i-th chunk is.
+  static __device__ __forceinline__ void place(int i, int& r, int& c) {
+    const int q = i * kThreads + (int)threadIdx.x;
+    r = q / kRowChunks;
+    c = (q % kRowChunks) ^ swizzle(r);
+  }
+
+  // first: first element of the tile; valid_: its rows or columns that exist, at least 1.
+  __device__ __forceinline__ void init(const T* first, int64_t ld_, int64_t valid_) {
+    base = (const char*)first;
+    ld = ld_ * kSize;
+    step = kCol ? ld * kDepth : (int64_t)kDepth * kSize;
+    valid = (int)min(valid_, (int64_t)kB);
+    if constexpr (kDirect) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        int r, c;
+        place(i, r, c);
+        offset[i] = kCol ? (uint32_t)r * (uint32_t)ld + (uint32_t)(min(c * kChunk, valid - kChunk) * kSize)
+                         : (uint32_t)min(r, valid - 1) * (uint32_t)ld + (uint32_t)c * 16u;
+      }
+    }
+  }
+
+  // Brings the step's chunks into LDS without passing registers; `left` = terms of the contraction that remain.
+  __device__ __forceinline__ void load_direct(lds_char* lds, int64_t left) {
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7FFFFFFF, 0x00020000);
+    lds_char* at = lds + __builtin_amdgcn_readfirstlane((int)threadIdx.x & ~63) * 16;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      uint32_t o = offset[i];
+      if (left < kDepth) {
+        int r, c;
+        place(i, r, c);
+        if ((kCol ? r : c * kChunk) >= left) o = kNowhere;
+      }
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(at + i * kThreads * 16), 16, (int)o, 0, 0, 0);
+    }
+    base += step;
+  }
+
+  // The same for rows at any alignment and of any length, through registers.
+  __device__ __forceinline__ void load_loose(Chunk (&regs)[kPer], int64_t left) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      int r, c;
+      place(i, r, c);
+      // elements of the chunk that exist
+      const int64_t there = kCol ? (r < left ? (int64_t)valid - c * kChunk : 0) : left - c * kChunk;
+      const T* p = (const T*)(base + (int64_t)(kCol ? r : min(r, valid - 1)) * ld) + c * kChunk;
+      if (there >= kChunk) {
+        regs[i] = *reinterpret_cast<const typename Pack<T, kChunk, false>::type*>(p);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kChunk; ++e) regs[i][e] = e < there ? p[e] : (T)0.f;
+      }
+    }
+    base += step;
+  }
+  static __device__ __forceinline__ void put(char* lds, const Chunk (&regs)[kPer]) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) *reinterpret_cast<Chunk*>(lds + (i * kThreads + (int)threadIdx.x) * 16) = regs[i];
+  }
+
+  // Fragment of 16 rows or columns from `at` on, half `h` of the step's terms.
+  static __device__ __forceinline__ typename Mfma<T>::frag fragment(const char* lds, int at, int h) {
+    using Frag = typename Mfma<T>::frag;
+    const int lane = threadIdx.x & 63, low = lane & 15, high = lane >> 4;
+    if constexpr (!kCol) {
+      const int r = at + low;
+      return *reinterpret_cast<const Frag*>(lds + r * 128 + (((h * 4 + high) ^ swizzle(r)) << 4));
+    } else if constexpr (kSize == 2) {
+      Frag f;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int r = h * 32 + high * 8 + q * 4 + (low >> 2);
+        const int byte = (at + (low & 3) * 4) * 2;
+        const short4_t v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) short4_t*)(lds + r * (kB * 2) + (byte ^ (swizzle(r) << 4))));
+        const auto t = __builtin_bit_cast(typename Pack<T, 4, true>::type, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[q * 4 + e] = t[e];
+      }
+      return f;
+    } else {
+      Frag f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = h * 16 + high * 4 + e;
+        f[e] = *reinterpret_cast<const float*>(lds + r * (kB * 4) + (((at + low) * 4) ^ (swizzle(r) << 4)));
+      }
+      return f;
+    }
+  }
+};
+
+// Workgroup -> output tile: the tiles in use are cut into one contiguous stretch for each XCD, so that the tiles that an
+// XCD works on at a time share rows of x and columns of w in its L2.
+__device__ __forceinline__ int64_t xcd_tile(int64_t tiles) {
+  const int64_t per = (tiles + kXcds - 1) / kXcds, b = blockIdx.x;
+  const int64_t t = (b % kXcds) * per + b / kXcds;
+  return b / kXcds < per && t < tiles ? t : -1;
+}
+
+template <class T, class TO, int kMode, int kBM, int kBN, int kWM, int kWN, bool kDirect>
+__global__ __launch_bounds__(64 * kWM * kWN, 2) void grouped_tile_kernel(GroupedArgs g, int col_tiles) {
+  constexpr int kThreads = 64 * kWM * kWN;
+  using OpA = Operand<T, kMode == kGradW, kBM, kThreads, kDirect>;
+  using OpB = Operand<T, kMode != kForward, kBN, kThreads, kDirect>;
+  using Frag = typename Mfma<T>::frag;
+  constexpr int FM = kBM / kWM / 16, FN = kBN / kWN / 16, kDepth = OpA::kDepth;
+  constexpr int kStage = OpA::kBytes + OpB::kBytes;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+
+  // the tile of the output, its operands, the length of the contraction
+  int64_t e, row0 = 0, end = 0, depth, m_left, n_left;
+  const int n_out = kMode == kForward ? g.m : g.k;
+  OpA a;
+  OpB b;
+  TO* c;
+  if constexpr (kMode == kGradW) {
+    const int row_tiles = (g.m + kBM - 1) / kBM;
+    const int64_t t = xcd_tile(g.groups * row_tiles * col_tiles);
+    if (t < 0) return;
+    e = t / (row_tiles * col_tiles);
+    const int in = (int)(t - e * row_tiles * col_tiles), mt = in / col_tiles, nt = in - mt * col_tiles;
+    group_rows_of(g, e, row0, end);
+    depth = end - row0;
+    m_left = g.m - (int64_t)mt * kBM;
+    n_left = n_out - (int64_t)nt * kBN;
+    a.init((const T*)g.a + row0 * g.lda + (int64_t)mt * kBM, g.lda, m_left);
+    b.init((const T*)g.b + row0 * g.ldb + (int64_t)nt * kBN, g.ldb, n_left);
+    c = (TO*)g.c + e * g.stride_c + (int64_t)mt * kBM * g.ldc + (int64_t)nt * kBN;
+  } else {
+    const int64_t row_tiles = count_row_tiles(g, kBM);
+    const int64_t t = xcd_tile(row_tiles * col_tiles);
+    if (t < 0) return;
+    const int64_t rt = t / col_tiles;
+    const int nt = (int)(t - rt * col_tiles);
+    if (!find_row_tile(g, rt, kBM, e, row0, end)) return;
+    depth = kMode == kForward ? g.k : g.m;
+    m_left = end - row0;
+    n_left = n_out - (int64_t)nt * kBN;
+    a.init((const T*)g.a + row0 * g.lda, g.lda, m_left);
+    const T* w = (const T*)g.b + e * g.stride_b;
+    b.init(kMode == kForward ? w + (int64_t)nt * kBN * g.ldb : w + (int64_t)nt * kBN, g.ldb, n_left);
+    c = (TO*)g.c + row0 * g.ldc + (int64_t)nt * kBN;
+  }
+
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int am = wave / kWN * (kBM / kWM), bn = wave % kWN * (kBN / kWN);
+  float4_t acc[FM][FN] = {};
+  auto multiply = [&](const char* lds) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      Frag fa[FM], fb[FN];
+#pragma unroll
+      for (int i = 0; i < FM; ++i) fa[i] = OpA::fragment(lds, am + i * 16, h);
+#pragma unroll
+      for (int j = 0; j < FN; ++j) fb[j] = OpB::fragment(lds + OpA::kBytes, bn + j * 16, h);
+      __builtin_amdgcn_sched_barrier(0);
+      // (the operands exchanged: a lane then holds four neighbouring columns of one row of the output)
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = Mfma<T>::mul(fb[j], fa[i], acc[i][j]);
+    }
+  };
+
+  // Two steps in LDS: one is multiplied while the next one is on its way.  The barrier at the head of a step says that
+  // its operands are there, and that nobody reads the other buffer any more.
+  const int64_t steps = (depth + kDepth - 1) / kDepth;
+  typename OpA::Chunk ra[kDirect ? 1 : OpA::kPer];
+  typename OpB::Chunk rb[kDirect ? 1 : OpB::kPer];
+  auto bring = [&](int64_t s) {
+    if constexpr (kDirect) {
+      lds_char* to = (lds_char*)lds + (s & 1) * kStage;
+      a.load_direct(to, depth - s * kDepth);
+      b.load_direct(to + OpA::kBytes, depth - s * kDepth);
+    } else {
+      a.load_loose(ra, depth - s * kDepth);
+      b.load_loose(rb, depth - s * kDepth);
+    }
+  };
+  auto land = [&](int64_t s) {
+    if constexpr (!kDirect) {
+      OpA::put(lds + (s & 1) * kStage, ra);
+      OpB::put(lds + (s & 1) * kStage + OpA::kBytes, rb);
+    }
+  };
+  if (steps > 0) {
+    bring(0);
+    land(0);
+  }
+  for (int64_t s = 0; s < steps; ++s) {
+    if constexpr (kDirect) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (s + 1 < steps) bring(s + 1);
+    multiply(lds + (s & 1) * kStage);
+    if (s + 1 < steps) land(s + 1);
+  }
+
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int row = am + i * 16 + (lane & 15);
+    if (row >= m_left) continue;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int col = bn + j * 16 + (lane >> 4) * 4;
+      TO* at = c + (int64_t)row * g.ldc + col;
+      if (col + 4 <= n_left) {
+        float v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = acc[i][j][q];
+        if (kMode == kGradW && g.accumulate) {
+          const auto old = *reinterpret_cast<const typename Pack<TO, 4, false>::type*>(at);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) v[q] += (float)old[q];
+        }
+        store_n<false, TO, 4>(at, v);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (col + q < n_left) at[q] = (TO)(acc[i][j][q] + (kMode == kGradW && g.accumulate ? (float)at[q] : 0.f));
+      }
+    }
+  }
+}
+
+}  // namespace hpspmm

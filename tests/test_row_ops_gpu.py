@@ -341,6 +341,13 @@ def test_grouped_products(pkg, gpu, kind, layout, how, rows, groups, k, m):
         one.check_around()
 
 
+@pytest.mark.parametrize("kind", ["bfloat16", "float16"])
+@pytest.mark.parametrize("how", ["ragged", "one"])
+@pytest.mark.parametrize("rows, groups, k, m", [(4500, 6, 264, 520), (9001, 3, 72, 1032), (5000, 40, 136, 64)])
+def test_grouped_products_of_many_rows(pkg, gpu, kind, how, rows, groups, k, m):
+    test_grouped_products(pkg, gpu, kind, "aligned_slice", how, rows, groups, k, m)
+
+
 @pytest.mark.parametrize("kind", ["bfloat16", "float32"])
 def test_grouped_products_with_offsets_that_are_none(pkg, gpu, kind):
     """Offsets that decrease, are negative or lie beyond the rows: unspecified values, but nothing around is touched."""
