@@ -52,10 +52,10 @@ __device__ __forceinline__ int64_t count_row_tiles(const GroupedArgs& g, int bm)
   return __builtin_amdgcn_readfirstlane(tiles);
 }
 
-// The group and first row of row tile `tile` (tiles of `bm` rows, each group starts a tile of its own); false when
-// there are fewer tiles.  Every wavefront looks for itself, 64 groups a step.
-__device__ __forceinline__ bool find_row_tile(const GroupedArgs& g, int64_t tile, int bm, int64_t& e, int64_t& row0,
-                                              int64_t& end) {
+// The group of row tile `tile` (tiles of `bm` rows, each group starts a tile of its own), its rows [begin, end) and its
+// first tile; false when there are fewer tiles.  Every wavefront looks for itself, 64 groups a step.
+__device__ __forceinline__ bool find_group(const GroupedArgs& g, int64_t tile, int bm, int64_t& e, int64_t& begin,
+                                           int64_t& end, int64_t& first) {
   const int lane = threadIdx.x & 63;
   int64_t before = 0;
   for (int64_t base = 0; base < g.groups; base += 64) {
@@ -72,15 +72,25 @@ __device__ __forceinline__ bool find_row_tile(const GroupedArgs& g, int64_t tile
     if (past) {
       const int at = __ffsll((unsigned long long)past) - 1;
       e = base + at;
-      const int64_t begin = uniform64(__shfl(b, at, 64));
+      begin = uniform64(__shfl(b, at, 64));
       end = uniform64(__shfl(f, at, 64));
-      const int first = __builtin_amdgcn_readfirstlane(__shfl(upto - tiles, at, 64));
-      row0 = begin + (tile - before - first) * bm;
+      first = before + __builtin_amdgcn_readfirstlane(__shfl(upto - tiles, at, 64));
       return true;
     }
     before += __builtin_amdgcn_readfirstlane(__shfl(upto, 63, 64));
   }
   return false;
+}
+
+// Tile `t` of a matrix of row_tiles x col_tiles output tiles, walked in panels of kPanel columns, row by row within a
+// panel: the tiles that are worked on at a time form a block, whose strips of the operands are shared.
+constexpr int kPanel = 8;
+__device__ __forceinline__ void panel_tile(int64_t t, int64_t row_tiles, int col_tiles, int64_t& row, int& col) {
+  const int64_t panel = t / (row_tiles * kPanel);
+  const int left = col_tiles - (int)panel * kPanel, wide = left < kPanel ? left : kPanel;
+  const int64_t in = t - panel * row_tiles * kPanel;
+  row = in / wide;
+  col = (int)panel * kPanel + (int)(in - row * wide);
 }
 
 }  // namespace hpspmm

@@ -41,7 +41,7 @@ bool chunked(const void* p, int64_t ld, int64_t stride, int64_t width, int64_t s
   return aligned_to(p, 16) && ld * size % 16 == 0 && stride * size % 16 == 0 && width * size % 16 == 0 && ld < ((int64_t)1 << 21);
 }
 
-template <class T, class TO, int kMode, int kBM, int kBN, int kWM, int kWN, bool kDirect>
+template <class T, class TO, int kMode, int kBM, int kBN, int kWM, int kWN, bool kDirect, int kC, int kStages>
 int launch_tiles(const hpspmm::GroupedArgs& g, hipStream_t st) {
   const int64_t n_out = kMode == hpspmm::kForward ? g.m : g.k;
   const int64_t col_tiles = ceil_div(n_out, kBN);
@@ -49,7 +49,7 @@ int launch_tiles(const hpspmm::GroupedArgs& g, hipStream_t st) {
   const int64_t tiles = ceil_div(row_tiles * col_tiles, hpspmm::kXcds) * hpspmm::kXcds;
   if (tiles == 0) return HPSPMM_OK;
   if (tiles > INT32_MAX / (64 * kWM * kWN)) return fail(HPSPMM_ERR_INVALID_ARG, "the product has too many output tiles");
-  hipLaunchKernelGGL((hpspmm::grouped_tile_kernel<T, TO, kMode, kBM, kBN, kWM, kWN, kDirect>), dim3((unsigned)tiles),
+  hipLaunchKernelGGL((hpspmm::grouped_tile_kernel<T, TO, kMode, kBM, kBN, kWM, kWN, kDirect, kC, kStages>), dim3((unsigned)tiles),
                      dim3(64 * kWM * kWN), 0, st, g, (int)col_tiles);
   return HPSPMM_OK;
 }
@@ -64,11 +64,11 @@ int launch_grouped(const hpspmm::GroupedArgs& g, int dtype, int out_type, hipStr
     return dispatch_dtype(out_type, [&](auto o) {
       using TO = decltype(o);
       if constexpr (std::is_same_v<T, TO> || (kMode == hpspmm::kGradW && std::is_same_v<TO, float>)) {
-        if (!direct) return launch_tiles<T, TO, kMode, 128, 128, 2, 2, false>(g, st);
+        if (!direct) return launch_tiles<T, TO, kMode, 128, 128, 2, 2, false, 8, 2>(g, st);
         if constexpr (sizeof(T) == 2) {
-          if (g.rows >= 4096) return launch_tiles<T, TO, kMode, 256, 256, 2, 4, true>(g, st);
+          if (g.rows >= 4096) return launch_tiles<T, TO, kMode, 256, 256, 2, 4, true, 8, 2>(g, st);
         }
-        return launch_tiles<T, TO, kMode, 128, 128, 2, 2, true>(g, st);
+        return launch_tiles<T, TO, kMode, 128, 128, 2, 2, true, 8, 2>(g, st);
       } else {
         return fail(HPSPMM_ERR_INVALID_ARG, "no product of these types");
       }

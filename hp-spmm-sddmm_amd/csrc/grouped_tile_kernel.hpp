@@ -47,18 +47,18 @@ struct Mfma<float> {
 };
 
 typedef __attribute__((address_space(3))) char lds_char;
-typedef __attribute__((address_space(3))) void lds_void;
 typedef short short4_t __attribute__((ext_vector_type(4)));
 
 // One operand of one output tile.
-template <class T, bool kCol, int kB, int kThreads, bool kDirect>
+// kC: 16-byte chunks of the contraction a step (4 or 8).
+template <class T, bool kCol, int kB, int kThreads, bool kDirect, int kC>
 struct Operand {
   static constexpr int kSize = (int)sizeof(T);
   static constexpr int kChunk = 16 / kSize;    // elements of a 16-byte chunk
-  static constexpr int kDepth = 8 * kChunk;    // terms of the contraction a step
-  static constexpr int kBytes = kB * 128;      // of LDS a step
-  static constexpr int kPer = kB * 8 / kThreads;  // chunks a thread brings in a step
-  static constexpr int kRowChunks = kCol ? kB / kChunk : 8;  // chunks of a row in LDS
+  static constexpr int kDepth = kC * kChunk;   // terms of the contraction a step
+  static constexpr int kBytes = kB * kC * 16;  // of LDS a step
+  static constexpr int kPer = kB * kC / kThreads;  // chunks a thread brings in a step
+  static constexpr int kRowChunks = kCol ? kB / kChunk : kC;  // chunks of a row in LDS
   static constexpr uint32_t kNowhere = 0xFFFFFFF0u;  // an offset beyond the buffer: the load gives zeros
   using Chunk = typename Pack<T, kChunk, true>::type;
 
@@ -69,7 +69,7 @@ struct Operand {
   uint32_t offset[kDirect ? kPer : 1];
 
   static __device__ __forceinline__ int swizzle(int r) {
-    if constexpr (!kCol) return r & 7;
+    if constexpr (!kCol) return kC == 8 ? r & 7 : (r >> 2) & 3;
     else if constexpr (kSize == 2) return ((r & 3) | ((r >> 1) & 4)) << 1;
     else return ((r >> 2) & 3) << 2;
   }
@@ -97,21 +97,29 @@ struct Operand {
     }
   }
 
-  // Brings the step's chunks into LDS without passing registers; `left` = terms of the contraction that remain.
-  __device__ __forceinline__ void load_direct(lds_char* lds, int64_t left) {
-    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7FFFFFFF, 0x00020000);
-    lds_char* at = lds + __builtin_amdgcn_readfirstlane((int)threadIdx.x & ~63) * 16;
+  // Before the first load of a step of which only `left` terms are left: what lies behind them becomes zeros, in this
+  // step and all later ones.
+  __device__ __forceinline__ void end_after(int64_t left) {
+    if (left >= kDepth) return;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      uint32_t o = offset[i];
-      if (left < kDepth) {
-        int r, c;
-        place(i, r, c);
-        if ((kCol ? r : c * kChunk) >= left) o = kNowhere;
-      }
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(at + i * kThreads * 16), 16, (int)o, 0, 0, 0);
+      int r, c;
+      place(i, r, c);
+      if ((kCol ? r : c * kChunk) >= left) offset[i] = kNowhere;
     }
-    base += step;
+  }
+  // Brings this thread's i-th chunk of a step into LDS without passing registers: a wavefront's 64 chunks land one behind
+  // the other.  (Written out: behind the builtin the compiler lets every transposed read of LDS wait for all loads that
+  // are under way.  The load has no output register; wait_loads() waits
+  // for it.  One wait state lies between the write of m0 and its use.)
+  __device__ __forceinline__ void load_direct(uint32_t lds, int i) const {
+    typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
+    const uint64_t at = (uint64_t)base;
+    const uint4_t rsrc = {(uint32_t)at, (uint32_t)(at >> 32) & 0xFFFFu, 0x7FFFFFFFu, 0x00020000u};
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(lds + i * kThreads * 16), "v"(offset[i]), "s"(rsrc)
+                 : "memory", "m0");
   }
 
   // The same for rows at any alignment and of any length, through registers.
@@ -143,7 +151,7 @@ struct Operand {
     const int lane = threadIdx.x & 63, low = lane & 15, high = lane >> 4;
     if constexpr (!kCol) {
       const int r = at + low;
-      return *reinterpret_cast<const Frag*>(lds + r * 128 + (((h * 4 + high) ^ swizzle(r)) << 4));
+      return *reinterpret_cast<const Frag*>(lds + r * (kC * 16) + (((h * 4 + high) ^ swizzle(r)) << 4));
     } else if constexpr (kSize == 2) {
       Frag f;
 #pragma unroll
@@ -169,6 +177,18 @@ struct Operand {
   }
 };
 
+// Waits until at most n of the loads that this wavefront has asked for are under way, and none of its reads of LDS.
+template <int n>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(n >= 0 && n < 64, "six bits count them");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(n) : "memory");
+}
+// A barrier that waits for no loads by itself.
+__device__ __forceinline__ void meet() {
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // Workgroup -> output tile: the tiles in use are cut into one contiguous stretch for each XCD, so that the tiles that an
 // XCD works on at a time share rows of x and columns of w in its L2.
 __device__ __forceinline__ int64_t xcd_tile(int64_t tiles) {
@@ -177,15 +197,15 @@ __device__ __forceinline__ int64_t xcd_tile(int64_t tiles) {
   return b / kXcds < per && t < tiles ? t : -1;
 }
 
-template <class T, class TO, int kMode, int kBM, int kBN, int kWM, int kWN, bool kDirect>
+template <class T, class TO, int kMode, int kBM, int kBN, int kWM, int kWN, bool kDirect, int kC, int kStages>
 __global__ __launch_bounds__(64 * kWM * kWN, 2) void grouped_tile_kernel(GroupedArgs g, int col_tiles) {
   constexpr int kThreads = 64 * kWM * kWN;
-  using OpA = Operand<T, kMode == kGradW, kBM, kThreads, kDirect>;
-  using OpB = Operand<T, kMode != kForward, kBN, kThreads, kDirect>;
+  using OpA = Operand<T, kMode == kGradW, kBM, kThreads, kDirect, kC>;
+  using OpB = Operand<T, kMode != kForward, kBN, kThreads, kDirect, kC>;
   using Frag = typename Mfma<T>::frag;
   constexpr int FM = kBM / kWM / 16, FN = kBN / kWN / 16, kDepth = OpA::kDepth;
   constexpr int kStage = OpA::kBytes + OpB::kBytes;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+  __shared__ __attribute__((aligned(1024))) char lds[kStages * kStage];
 
   // the tile of the output, its operands, the length of the contraction
   int64_t e, row0 = 0, end = 0, depth, m_left, n_left;
@@ -198,21 +218,25 @@ __global__ __launch_bounds__(64 * kWM * kWN, 2) void grouped_tile_kernel(Grouped
     const int64_t t = xcd_tile(g.groups * row_tiles * col_tiles);
     if (t < 0) return;
     e = t / (row_tiles * col_tiles);
-    const int in = (int)(t - e * row_tiles * col_tiles), mt = in / col_tiles, nt = in - mt * col_tiles;
+    int64_t mt;
+    int nt;
+    panel_tile(t - e * row_tiles * col_tiles, row_tiles, col_tiles, mt, nt);
     group_rows_of(g, e, row0, end);
     depth = end - row0;
-    m_left = g.m - (int64_t)mt * kBM;
+    m_left = g.m - mt * kBM;
     n_left = n_out - (int64_t)nt * kBN;
-    a.init((const T*)g.a + row0 * g.lda + (int64_t)mt * kBM, g.lda, m_left);
+    a.init((const T*)g.a + row0 * g.lda + mt * kBM, g.lda, m_left);
     b.init((const T*)g.b + row0 * g.ldb + (int64_t)nt * kBN, g.ldb, n_left);
-    c = (TO*)g.c + e * g.stride_c + (int64_t)mt * kBM * g.ldc + (int64_t)nt * kBN;
+    c = (TO*)g.c + e * g.stride_c + mt * kBM * g.ldc + (int64_t)nt * kBN;
   } else {
     const int64_t row_tiles = count_row_tiles(g, kBM);
     const int64_t t = xcd_tile(row_tiles * col_tiles);
     if (t < 0) return;
-    const int64_t rt = t / col_tiles;
-    const int nt = (int)(t - rt * col_tiles);
-    if (!find_row_tile(g, rt, kBM, e, row0, end)) return;
+    int64_t first, mt;
+    int nt;
+    if (!find_group(g, t / col_tiles, kBM, e, row0, end, first)) return;
+    panel_tile(t - first * col_tiles, (end - row0 + kBM - 1) / kBM, col_tiles, mt, nt);
+    row0 += mt * kBM;
     depth = kMode == kForward ? g.k : g.m;
     m_left = end - row0;
     n_left = n_out - (int64_t)nt * kBN;
@@ -225,55 +249,97 @@ __global__ __launch_bounds__(64 * kWM * kWN, 2) void grouped_tile_kernel(Grouped
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int am = wave / kWN * (kBM / kWM), bn = wave % kWN * (kBN / kWN);
   float4_t acc[FM][FN] = {};
-  auto multiply = [&](const char* lds) {
+  // The products of one step, sum by sum of 16 rows; `between(i)` after the i-th.  The next half of the step is read
+  // while this one is multiplied.
+  constexpr int H = kC / 4;
+  auto multiply = [&](const char* lds, auto between) {
+    Frag fa[H][FM], fb[H][FN];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      Frag fa[FM], fb[FN];
+    for (int j = 0; j < FN; ++j) fb[0][j] = OpB::fragment(lds + OpA::kBytes, bn + j * 16, 0);
 #pragma unroll
-      for (int i = 0; i < FM; ++i) fa[i] = OpA::fragment(lds, am + i * 16, h);
+    for (int i = 0; i < FM; ++i) fa[0][i] = OpA::fragment(lds, am + i * 16, 0);
 #pragma unroll
-      for (int j = 0; j < FN; ++j) fb[j] = OpB::fragment(lds + OpA::kBytes, bn + j * 16, h);
-      __builtin_amdgcn_sched_barrier(0);
-      // (the operands exchanged: a lane then holds four neighbouring columns of one row of the output)
+    for (int h = 0; h < H; ++h)
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
+      for (int i = 0; i < FM; ++i) {
+        // (the operands exchanged: a lane then holds four neighbouring columns of one row of the output)
 #pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = Mfma<T>::mul(fb[j], fa[i], acc[i][j]);
-    }
+        for (int j = 0; j < FN; ++j) acc[i][j] = Mfma<T>::mul(fb[h][j], fa[h][i], acc[i][j]);
+        between(h * FM + i);
+        if (h + 1 < H) {
+          fa[h + 1][i] = OpA::fragment(lds, am + i * 16, h + 1);
+          if (i < FN) fb[h + 1][i] = OpB::fragment(lds + OpA::kBytes, bn + i * 16, h + 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
   };
 
-  // Two steps in LDS: one is multiplied while the next one is on its way.  The barrier at the head of a step says that
-  // its operands are there, and that nobody reads the other buffer any more.
+  // kStages steps in LDS: one is multiplied while the next ones are on their way.  The barrier at the head of a step says
+  // that its operands are there, and that nobody reads the stage before it any more, which the step brought in then
+  // takes.  Loads past the registers are counted: those of the kStages - 2 steps behind may still be under way (steps
+  // beyond the last one are asked for as well, as zeros, so that the count holds to the end).
+  static_assert(kDirect || kStages == 2, "loads through registers are one step ahead");
   const int64_t steps = (depth + kDepth - 1) / kDepth;
   typename OpA::Chunk ra[kDirect ? 1 : OpA::kPer];
   typename OpB::Chunk rb[kDirect ? 1 : OpB::kPer];
-  auto bring = [&](int64_t s) {
-    if constexpr (kDirect) {
-      lds_char* to = (lds_char*)lds + (s & 1) * kStage;
-      a.load_direct(to, depth - s * kDepth);
-      b.load_direct(to + OpA::kBytes, depth - s * kDepth);
-    } else {
-      a.load_loose(ra, depth - s * kDepth);
-      b.load_loose(rb, depth - s * kDepth);
-    }
-  };
-  auto land = [&](int64_t s) {
-    if constexpr (!kDirect) {
-      OpA::put(lds + (s & 1) * kStage, ra);
-      OpB::put(lds + (s & 1) * kStage + OpA::kBytes, rb);
-    }
+  const uint32_t lds_wave = (uint32_t)(uintptr_t)(lds_char*)lds + (uint32_t)wave * 1024u;  // where this wavefront's chunks go
+  constexpr int kLoads = OpA::kPer + OpB::kPer;
+  static_assert(FN <= FM, "the fragments of a half are read between the sums of the half before");
+  auto bring_direct = [&](int stage, int i) {
+    const uint32_t to = lds_wave + (uint32_t)(stage * kStage);
+    if (i < OpA::kPer) a.load_direct(to, i);
+    else b.load_direct(to + OpA::kBytes, i - OpA::kPer);
   };
   if (steps > 0) {
-    bring(0);
-    land(0);
+    if constexpr (kDirect) {
+      for (int s = 0; s < kStages - 1; ++s) {
+        a.end_after(depth - s * kDepth);
+        b.end_after(depth - s * kDepth);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) bring_direct(s, i);
+        a.base += a.step;
+        b.base += b.step;
+      }
+    } else {
+      a.load_loose(ra, depth);
+      b.load_loose(rb, depth);
+      OpA::put(lds, ra);
+      OpB::put(lds + OpA::kBytes, rb);
+    }
   }
+  int stage = 0;
   for (int64_t s = 0; s < steps; ++s) {
-    if constexpr (kDirect) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (s + 1 < steps) bring(s + 1);
-    multiply(lds + (s & 1) * kStage);
-    if (s + 1 < steps) land(s + 1);
+    const int before = stage == 0 ? kStages - 1 : stage - 1;
+    if constexpr (kDirect) {
+      wait_loads<(kStages - 2) * kLoads>();
+      meet();
+      a.end_after(depth - (s + kStages - 1) * kDepth);
+      b.end_after(depth - (s + kStages - 1) * kDepth);
+      // the loads spread over the products: asked for in one go they would keep the wavefront waiting for its turn
+      multiply(lds + stage * kStage, [&](int i) {
+        constexpr int kSpread = 8;
+#pragma unroll
+        for (int q = 0; q < kSpread; ++q)
+          if (i * kSpread + q < kLoads) bring_direct(before, i * kSpread + q);
+      });
+      a.base += a.step;
+      b.base += b.step;
+    } else {
+      __syncthreads();
+      if (s + 1 < steps) {
+        a.load_loose(ra, depth - (s + 1) * kDepth);
+        b.load_loose(rb, depth - (s + 1) * kDepth);
+      }
+      multiply(lds + stage * kStage, [](int) {});
+      if (s + 1 < steps) {
+        OpA::put(lds + before * kStage, ra);
+        OpB::put(lds + before * kStage + OpA::kBytes, rb);
+      }
+    }
+    stage = stage + 1 == kStages ? 0 : stage + 1;
   }
+  // (nothing may be on its way into LDS when the workgroup ends)
+  if constexpr (kDirect) wait_loads<0>();
 
   const int lane = threadIdx.x & 63;
 #pragma unroll
