@@ -55,15 +55,10 @@ __global__ __launch_bounds__(kBlock) void embedding_lookup_kernel(int64_t n, uin
   }
 }
 
-// keys[i] = id of row i (or `ids` when it is outside [0, ids)), vals[i] = i.
-template <class Id>
-__global__ __launch_bounds__(kBlock) void row_keys_kernel(int64_t n, uint32_t ids, const Id* __restrict__ id,
-                                                         uint32_t* __restrict__ keys, int32_t* __restrict__ vals) {
-  const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-  if (i >= n) return;
-  keys[i] = id_key(id[i], ids);
-  vals[i] = (int32_t)i;
-}
+// ---------------------------------------------------------------------------------------------
+// Rows sorted by id: keys[q] / vals[q] = id and row of the q-th row in that order, rows of one id in increasing order,
+// ids outside [0, ids) as key `ids` behind all others.
+// ---------------------------------------------------------------------------------------------
 
 // First position of the sorted keys that is not below `key`.
 __device__ __forceinline__ int64_t lower_bound_u32(const uint32_t* __restrict__ keys, int64_t n, uint32_t key) {
@@ -76,34 +71,407 @@ __device__ __forceinline__ int64_t lower_bound_u32(const uint32_t* __restrict__ 
   return lo;
 }
 
-// offsets[g] = rows whose key is below g, g = 0 ... groups; order[i] = the sorted rows.
+// offsets[g] = rows whose key is below g, g = 0 ... groups.
 HPSPMM_KERNEL __launch_bounds__(kBlock) void row_offsets_kernel(int64_t n, int64_t groups,
                                                              const uint32_t* __restrict__ keys,
-                                                             const int32_t* __restrict__ vals,
-                                                             int32_t* __restrict__ order,
                                                              int32_t* __restrict__ offsets) {
-  const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-  if (i <= groups) offsets[i] = (int32_t)lower_bound_u32(keys, n, (uint32_t)i);
-  if (i < n) order[i] = vals[i];
+  const int64_t g = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  if (g <= groups) offsets[g] = (int32_t)lower_bound_u32(keys, n, (uint32_t)g);
 }
 
-// d_table[v, :] = (accumulate ? d_table[v, :] : 0) + scale * sum of the rows of `grad` whose key is v, in the order of
-// their positions.  One workgroup per row of the table and column tile.
-template <class T, class TO>
-__global__ __launch_bounds__(kBlock) void embedding_grad_kernel(int64_t n, int32_t width, const uint32_t* __restrict__ keys,
-                                                               const int32_t* __restrict__ pos,
-                                                               const T* __restrict__ grad, int64_t ld_grad, float scale,
-                                                               TO* __restrict__ d_table, int64_t ld_table,
-                                                               int accumulate) {
-  const uint32_t v = blockIdx.x;
-  const int64_t first = lower_bound_u32(keys, n, v), last = lower_bound_u32(keys, n, v + 1);
-  if (first == last && accumulate) return;
-  for (int c = (int)blockIdx.y * kBlock + (int)threadIdx.x; c < width; c += (int)gridDim.y * kBlock) {
-    float sum = 0.f;
-    for (int64_t q = first; q < last; ++q) sum += (float)grad[(int64_t)pos[q] * ld_grad + c];
-    TO* at = d_table + (int64_t)v * ld_table + c;
-    const float old = accumulate ? (float)*at : 0.f;
-    *at = (TO)(old + scale * sum);
+// Few rows: the place of a row is the number of rows before it, counted - n^2 comparisons, but one launch and no step
+// that waits for another.  A workgroup places 64 rows, one a lane; its 16 wavefronts count in a sixteenth of the rows
+// each, which they hold in LDS.  Rows n ... n + virtual - 1 are the group numbers 0 ...: their place is their offset.
+constexpr int kRankWaves = 16;
+constexpr int kRankMaxRows = 16384;
+template <class Id>
+__global__ __launch_bounds__(64 * kRankWaves) void row_rank_kernel(int32_t n, int32_t n_virtual, uint32_t ids,
+                                                                  const Id* __restrict__ id, uint32_t* __restrict__ keys,
+                                                                  int32_t* __restrict__ vals,
+                                                                  int32_t* __restrict__ offsets) {
+  __shared__ __attribute__((aligned(16))) uint32_t s_key[kRankMaxRows];
+  __shared__ int32_t s_count[kRankWaves][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int i0 = blockIdx.x * 64, i = i0 + lane;
+  const bool real = i < n;
+  const uint32_t key = real ? id_key(id[i], ids) : (uint32_t)(i - n);
+  // tiles of 64 rows, dealt to the wavefronts in stretches
+  const int tiles = (n + 63) / 64, per = (tiles + kRankWaves - 1) / kRankWaves;
+  const int first = wave * per, last = min(first + per, tiles);
+  uint32_t* mine = s_key + wave * per * 64;
+  for (int t = first; t < last; ++t) {
+    const int j = t * 64 + lane;
+    mine[(t - first) * 64 + lane] = j < n ? id_key(id[j], ids) : 0xFFFFFFFFu;
+  }
+  // (a wavefront reads what it has written itself: no barrier)
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  int count = 0;
+  for (int t = first; t < last; ++t) {
+    const uint4* at = reinterpret_cast<const uint4*>(mine + (t - first) * 64);
+    const int j0 = t * 64;
+    if (j0 == i0 && real) {
+#pragma unroll 4
+      for (int q = 0; q < 16; ++q) {
+        const uint4 v = at[q];
+        count += v.x < key + (uint32_t)(q * 4 + 0 < lane);
+        count += v.y < key + (uint32_t)(q * 4 + 1 < lane);
+        count += v.z < key + (uint32_t)(q * 4 + 2 < lane);
+        count += v.w < key + (uint32_t)(q * 4 + 3 < lane);
+      }
+    } else {
+      // rows of the same id count where they lie before this one
+      const uint32_t below = key + (uint32_t)(real && j0 < i0);
+#pragma unroll 4
+      for (int q = 0; q < 16; ++q) {
+        const uint4 v = at[q];
+        count += v.x < below;
+        count += v.y < below;
+        count += v.z < below;
+        count += v.w < below;
+      }
+    }
+  }
+  s_count[wave][lane] = count;
+  __syncthreads();
+  if (wave != 0) return;
+  count = 0;
+#pragma unroll
+  for (int w = 0; w < kRankWaves; ++w) count += s_count[w][lane];
+  if (real) {
+    if (keys) keys[count] = key;
+    vals[count] = i;
+  } else if (i - n < n_virtual) {
+    offsets[i - n] = count;
+  }
+}
+
+// Many rows: stable counting sort by digits of up to 10 bits, least significant first, two launches a digit: counts per
+// tile of rows, then the rows to their places.  A tile's rows go to the wavefronts in stretches of 4 x 64; a row's rank
+// among the equal digits of its stretch is found by ballots over the digit's bits.
+constexpr int kDigitBits = 10, kDigitBins = 1 << kDigitBits;
+constexpr int kDigitThreads = 512, kDigitWaves = kDigitThreads / 64, kDigitRounds = 4;
+constexpr int kDigitTile = kDigitThreads * kDigitRounds;
+constexpr int kDigitFused = 256;  // up to so many tiles every workgroup adds up the counts of the others itself
+
+// The key of row i of this pass: from the ids in the first one.
+template <class Id>
+struct RowKeys {
+  const Id* id;          // first pass
+  const uint32_t* keys;  // later ones
+  const int32_t* vals;
+  uint32_t ids;
+  __device__ __forceinline__ uint32_t key(int64_t i) const { return id ? id_key(id[i], ids) : keys[i]; }
+  __device__ __forceinline__ int32_t val(int64_t i) const { return id ? (int32_t)i : vals[i]; }
+};
+
+// hist[tile * bins + d] (or hist[d * tiles + tile], for a scan over all of it) = rows of the tile with digit d.
+template <class Id>
+__global__ __launch_bounds__(kDigitThreads) void digit_count_kernel(int64_t n, RowKeys<Id> rows, int shift, int bits,
+                                                                   int64_t tiles, int by_digit, uint32_t* __restrict__ hist) {
+  __shared__ uint32_t s_hist[kDigitBins];
+  const int bins = 1 << bits;
+  for (int d = threadIdx.x; d < bins; d += kDigitThreads) s_hist[d] = 0;
+  __syncthreads();
+  const int64_t base = (int64_t)blockIdx.x * kDigitTile;
+#pragma unroll
+  for (int q = 0; q < kDigitRounds; ++q) {
+    const int64_t i = base + q * kDigitThreads + threadIdx.x;
+    if (i < n) atomicAdd(&s_hist[(rows.key(i) >> shift) & (bins - 1)], 1u);
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < bins; d += kDigitThreads)
+    hist[by_digit ? (int64_t)d * tiles + blockIdx.x : (int64_t)blockIdx.x * bins + d] = s_hist[d];
+}
+
+// Row i of the tile goes to (rows with a lower digit) + (rows of the tiles before with this digit) + (its rank in the
+// tile).  scanned: hist holds the first two sums already; otherwise they are added up here.  offsets (only when one
+// digit is all there is): offsets[d] = rows with a digit below d, by the first workgroup.
+template <class Id>
+__global__ __launch_bounds__(kDigitThreads) void digit_scatter_kernel(int64_t n, RowKeys<Id> rows, int shift, int bits,
+                                                                     int64_t tiles, int scanned,
+                                                                     const uint32_t* __restrict__ hist,
+                                                                     uint32_t* __restrict__ keys_out,
+                                                                     int32_t* __restrict__ vals_out, int64_t groups,
+                                                                     int32_t* __restrict__ offsets) {
+  __shared__ uint32_t s_base[kDigitBins];
+  __shared__ uint32_t s_wave[kDigitWaves][kDigitBins];
+  __shared__ uint32_t s_sum[kDigitWaves];
+  const int bins = 1 << bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t tile = blockIdx.x, base = tile * kDigitTile;
+  for (int d = threadIdx.x; d < bins * kDigitWaves; d += kDigitThreads) s_wave[d >> bits][d & (bins - 1)] = 0;
+  __syncthreads();
+  // ranks within the wavefront's stretch (a wavefront counts in its own row of s_wave: no barrier in between)
+  uint32_t key[kDigitRounds], rank[kDigitRounds];
+  int32_t val[kDigitRounds];
+  const uint64_t below = (1ull << lane) - 1ull;
+#pragma unroll
+  for (int q = 0; q < kDigitRounds; ++q) {
+    const int64_t i = base + wave * (64 * kDigitRounds) + q * 64 + lane;
+    key[q] = i < n ? rows.key(i) : 0u;
+    val[q] = i < n ? rows.val(i) : 0;
+  }
+#pragma unroll
+  for (int q = 0; q < kDigitRounds; ++q) {
+    const int64_t i = base + wave * (64 * kDigitRounds) + q * 64 + lane;
+    const uint32_t d = (key[q] >> shift) & (bins - 1);
+    uint64_t same = __ballot(i < n);
+    for (int b = 0; b < bits; ++b) {
+      const uint64_t set = __ballot((d >> b) & 1u);
+      same &= ((d >> b) & 1u) ? set : ~set;
+    }
+    const uint32_t before = (uint32_t)__popcll(same & below);
+    rank[q] = s_wave[wave][d] + before;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (i < n && before == 0) s_wave[wave][d] += (uint32_t)__popcll(same);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+  // where the tile's rows of each digit begin
+  if (scanned) {
+    for (int d = threadIdx.x; d < bins; d += kDigitThreads) s_base[d] = hist[(int64_t)d * tiles + tile];
+  } else {
+    // (two bins a thread at most)
+    uint32_t all[2] = {0, 0}, earlier[2] = {0, 0};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int d = (int)threadIdx.x * 2 + h;
+      if (d < bins) {
+#pragma unroll 8
+        for (int64_t t = 0; t < tiles; ++t) {
+          const uint32_t c = hist[t * bins + d];
+          all[h] += c;
+          if (t < tile) earlier[h] += c;
+        }
+      }
+    }
+    uint32_t upto = all[0] + all[1];
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+      const uint32_t other = __shfl_up(upto, s, 64);
+      if (lane >= s) upto += other;
+    }
+    if (lane == 63) s_sum[wave] = upto;
+    __syncthreads();
+    uint32_t start = upto - all[0] - all[1];
+    for (int w = 0; w < wave; ++w) start += s_sum[w];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int d = (int)threadIdx.x * 2 + h;
+      if (d < bins) {
+        s_base[d] = start + earlier[h];
+        if (offsets && tile == 0 && d <= groups) offsets[d] = (int32_t)start;
+      }
+      start += all[h];
+    }
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < bins; d += kDigitThreads) {
+    uint32_t at = s_base[d];
+#pragma unroll
+    for (int w = 0; w < kDigitWaves; ++w) {
+      const uint32_t c = s_wave[w][d];
+      s_wave[w][d] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < kDigitRounds; ++q) {
+    const int64_t i = base + wave * (64 * kDigitRounds) + q * 64 + lane;
+    if (i >= n) continue;
+    const uint32_t to = s_wave[wave][(key[q] >> shift) & (bins - 1)] + rank[q];
+    if (keys_out) keys_out[to] = key[q];
+    vals_out[to] = val[q];
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Gradient of the lookup: sums over the stretches of equal keys of the sorted rows.  A chunk of 2^chunk_log2 sorted rows
+// is added up by one group of threads, 16 bytes of a row each; a sum that lies within the chunk goes to the table, one
+// that began before it to carry slot 2c, one that goes on behind it to slot 2c + 1 (32 bits), and a second kernel adds
+// those up in order.  No atomics: the same ids give the same bits.
+// ---------------------------------------------------------------------------------------------
+
+constexpr int kSumFlight = 8;  // rows in flight
+
+template <class T, bool kAligned>
+__device__ __forceinline__ void load_row(const T* p, int there, float (&v)[kPer16<T>]) {
+  if (there >= kPer16<T>) {
+    load16<kAligned>(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer16<T>; ++i) v[i] = i < there ? (float)p[i] : 0.f;
+  }
+}
+
+// at[0 .. there) = (accumulate ? at : 0) + scale * v.
+template <class TO, int kN, bool kAligned>
+__device__ __forceinline__ void store_sum(TO* at, int there, const float (&v)[kN], float scale, int accumulate) {
+  constexpr int kPart = kN < kPer16<TO> ? kN : kPer16<TO>;
+#pragma unroll
+  for (int p = 0; p < kN; p += kPart) {
+    float out[kPart];
+    if (there >= p + kPart) {
+      if (accumulate) {
+        const auto old = *reinterpret_cast<const typename Pack<TO, kPart, kAligned>::type*>(at + p);
+#pragma unroll
+        for (int i = 0; i < kPart; ++i) out[i] = (float)old[i] + scale * v[p + i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPart; ++i) out[i] = scale * v[p + i];
+      }
+      store_n<kAligned, TO, kPart>(at + p, out);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPart; ++i)
+        if (p + i < there) at[p + i] = (TO)((accumulate ? (float)at[p + i] : 0.f) + scale * v[p + i]);
+    }
+  }
+}
+
+struct SumArgs {
+  int64_t n;
+  uint32_t vocab;
+  int32_t width, pitch;  // columns; floats from one carry slot to the next
+  const uint32_t* keys;
+  const int32_t* pos;
+  const void* grad;
+  int64_t ld_grad;
+  float scale;
+  void* d_table;
+  int64_t ld_table;
+  int accumulate;
+  float* carry;
+  int chunk_log2, tpr_log2;
+  int64_t chunks;
+  unsigned sum_blocks;   // workgroups that add up
+  unsigned zero_blocks;  // workgroups behind them that fill the rows of the table that no id points at with zeros
+};
+
+constexpr int kZeroRows = 64;  // rows of the table a workgroup looks at for that
+
+template <class T, class TO, bool kAligned, bool kWide>
+__global__ __launch_bounds__(kBlock) void embedding_sum_kernel(SumArgs g) {
+  constexpr int V = kPer16<T>;
+  const int tpr = 1 << g.tpr_log2;
+  if (blockIdx.x >= g.sum_blocks) {
+    // (all column tiles of a row by one workgroup)
+    if (blockIdx.y != 0) return;
+    const int lane = threadIdx.x & 63;
+    constexpr int kPart = kPer16<TO>;
+    const float zero[kPart] = {};
+    for (int64_t v0 = (int64_t)(blockIdx.x - g.sum_blocks) * kZeroRows; v0 < g.vocab; v0 += (int64_t)g.zero_blocks * kZeroRows) {
+      bool empty = false;
+      if (v0 + lane < g.vocab) {
+        const int64_t at = lower_bound_u32(g.keys, g.n, (uint32_t)(v0 + lane));
+        empty = at == g.n || g.keys[at] != (uint32_t)(v0 + lane);
+      }
+      uint64_t rows = __ballot(empty);
+      while (rows) {
+        const int r = __ffsll((unsigned long long)rows) - 1;
+        rows &= rows - 1;
+        TO* row = (TO*)g.d_table + (v0 + r) * g.ld_table;
+        for (int c = (int)threadIdx.x * kPart; c < g.width; c += (int)blockDim.x * kPart)
+          store_sum<TO, kPart, kAligned>(row + c, g.width - c, zero, 0.f, 0);
+      }
+    }
+    return;
+  }
+  const int64_t c = kWide ? (int64_t)blockIdx.x : ((int64_t)blockIdx.x << (8 - g.tpr_log2)) + ((int)threadIdx.x >> g.tpr_log2);
+  const int col = ((int)blockIdx.y * tpr + ((int)threadIdx.x & (tpr - 1))) * V;
+  const int there = g.width - col;
+  if (c >= g.chunks || there <= 0) return;
+  const int64_t begin = c << g.chunk_log2, end = min(begin + ((int64_t)1 << g.chunk_log2), g.n);
+  uint32_t cur = g.keys[begin];
+  if (cur >= g.vocab) return;
+  bool open = begin > 0 && g.keys[begin - 1] == cur;  // the sum began in an earlier chunk
+  float acc[V] = {};
+  const T* grad = (const T*)g.grad + col;
+  auto close = [&](int slot) {
+    if (slot >= 0) {
+      float* at = g.carry + (2 * c + slot) * (int64_t)g.pitch + col;
+      store_sum<float, V, true>(at, g.pitch - col, acc, 1.f, 0);
+    } else {
+      store_sum<TO, V, kAligned>((TO*)g.d_table + (int64_t)cur * g.ld_table + col, there, acc, g.scale, g.accumulate);
+    }
+  };
+  bool done = false;
+  for (int64_t q0 = begin; q0 < end && !done; q0 += kSumFlight) {
+    uint32_t key[kSumFlight];
+    float row[kSumFlight][V];
+#pragma unroll
+    for (int u = 0; u < kSumFlight; ++u) {
+      key[u] = q0 + u < end ? g.keys[q0 + u] : g.vocab;
+      if (key[u] < g.vocab) load_row<T, kAligned>(grad + (int64_t)g.pos[q0 + u] * g.ld_grad, there, row[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kSumFlight; ++u) {
+      if (done) break;
+      if (key[u] != cur) {
+        // (behind the chunk's last row, the vocabulary's end stands for what follows)
+        if (q0 + u >= end) {
+          done = true;
+          break;
+        }
+        close(open ? 0 : -1);
+        open = false;
+        cur = key[u];
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = 0.f;
+        if (cur >= g.vocab) {
+          done = true;
+          break;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] += row[u][i];
+    }
+  }
+  if (cur >= g.vocab) return;
+  const bool goes_on = end < g.n && g.keys[end] == cur;
+  close(open ? 0 : goes_on ? 1 : -1);
+}
+
+// The sums that cross chunks: the chunk in which one begins adds up its slots.  A workgroup looks at kFixChunks chunks
+// and owns 256 columns; its wavefronts take a stretch of the slots each, and their sums are added in that order.
+constexpr int kFixChunks = 8;
+template <class TO, bool kAligned>
+__global__ __launch_bounds__(kBlock) void embedding_fix_kernel(SumArgs g) {
+  __shared__ float s_part[kWavesPerBlock][64][4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int col = ((int)blockIdx.y * 64 + lane) * 4, there = g.width - col;
+  for (int64_t c = (int64_t)blockIdx.x * kFixChunks; c < min((int64_t)(blockIdx.x + 1) * kFixChunks, g.chunks); ++c) {
+    const int64_t begin = c << g.chunk_log2, end = min(begin + ((int64_t)1 << g.chunk_log2), g.n);
+    if (end >= g.n) return;
+    const uint32_t key = g.keys[end - 1];
+    if (key >= g.vocab) return;
+    if (g.keys[end] != key) continue;                                                // it ends here
+    if (g.keys[begin] == key && begin > 0 && g.keys[begin - 1] == key) continue;     // it began earlier
+    const int64_t stop = lower_bound_u32(g.keys, g.n, key + 1);
+    const int64_t slots = ((stop - 1) >> g.chunk_log2) - c;  // chunks behind this one that it reaches
+    const int64_t per = (slots + kWavesPerBlock - 1) / kWavesPerBlock;
+    const int64_t first = wave * per, last = min(first + per, slots);
+    float acc[4] = {};
+    if (there > 0) {
+      if (wave == 0) load16<true>(g.carry + (2 * c + 1) * (int64_t)g.pitch + col, acc);
+#pragma unroll 8
+      for (int64_t s = first; s < last; ++s) {
+        float v[4];
+        load16<true>(g.carry + 2 * (c + 1 + s) * (int64_t)g.pitch + col, v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] += v[i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s_part[wave][lane][i] = acc[i];
+    __syncthreads();
+    if (wave == 0 && there > 0) {
+#pragma unroll
+      for (int w = 1; w < kWavesPerBlock; ++w)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] += s_part[w][lane][i];
+      store_sum<TO, 4, kAligned>((TO*)g.d_table + (int64_t)key * g.ld_table + col, there, acc, g.scale, g.accumulate);
+    }
+    __syncthreads();
   }
 }
 

@@ -55,18 +55,94 @@ int key_bits(int64_t ids) {
   return bits;
 }
 
-// The n rows sorted by id, ids outside [0, ids) last, rows of one id in increasing order: *cur = which of the plan's
-// buffers holds them.
-int sort_rows(hpspmm_rows_plan* plan, int64_t n, int64_t ids, const void* d_ids, int id_type, hipStream_t st, int* cur) {
-  *cur = 0;
-  if (n == 0) return HPSPMM_OK;
-  dispatch_id(id_type, [&](auto id) {
-    using Id = decltype(id);
-    hipLaunchKernelGGL((hpspmm::row_keys_kernel<Id>), dim3((unsigned)ceil_div(n, hpspmm::kBlock)), dim3(hpspmm::kBlock), 0,
-                       st, n, (uint32_t)ids, (const Id*)d_ids, plan->d_keys[0], plan->d_vals[0]);
-    return HPSPMM_OK;
-  });
-  return radix_sort_pairs(n, plan->d_keys, plan->d_vals, plan->d_hist, plan->d_scan, key_bits(ids), st, cur);
+// Digits of the counting sort for ids below `ids` (and the key `ids` itself): how many, of how many bits each.
+void key_digits(int64_t ids, int* digits, int* bits) {
+  const int all = key_bits(ids);
+  *digits = (int)ceil_div(all, hpspmm::kDigitBits);
+  *bits = (int)ceil_div(all, *digits);
+}
+
+// The n rows sorted by id, ids outside [0, ids) last, rows of one id in increasing order, in d_keys / d_vals
+// (hpspmm_group_rows: the rows straight to d_order, and the groups' offsets; keys are then kept only where it needs them).
+struct Sorted {
+  const uint32_t* keys;
+  const int32_t* rows;
+};
+int sort_rows(hpspmm_rows_plan* plan, int64_t n, int64_t ids, const void* d_ids, int id_type, int32_t* d_order,
+              int32_t* d_offsets, hipStream_t st, Sorted* out) {
+  using namespace hpspmm;
+  if (out) *out = {plan->d_keys[0], plan->d_vals[0]};
+  const int64_t n_offsets = d_offsets ? ids + 1 : 0;
+  // Counting ranks costs n^2 / 16 steps of a wavefront in all, digits two dependent launches each: 512 rows 5 us against
+  // 12, 8192 rows and 2^17 ids 10 against 20, about the same at 16384.
+  if (n <= kRankMaxRows && (n_offsets <= 4 * kRankMaxRows || n == 0)) {
+    const int64_t count = n + n_offsets;
+    if (count == 0) return HPSPMM_OK;
+    return dispatch_id(id_type, [&](auto id) {
+      using Id = decltype(id);
+      hipLaunchKernelGGL((row_rank_kernel<Id>), dim3((unsigned)ceil_div(count, 64)), dim3(64 * kRankWaves), 0, st, (int32_t)n,
+                         (int32_t)n_offsets, (uint32_t)ids, (const Id*)d_ids, d_order ? nullptr : plan->d_keys[0],
+                         d_order ? d_order : plan->d_vals[0], d_offsets);
+      return HPSPMM_OK;
+    });
+  }
+  int digits, bits;
+  key_digits(ids, &digits, &bits);
+  const int64_t tiles = ceil_div(n, kDigitTile);
+  const bool fused = tiles <= kDigitFused;
+  // offsets come with the only digit, or from the sorted keys
+  const bool with_offsets = d_offsets && digits == 1 && fused;
+  for (int p = 0; p < digits; ++p) {
+    const int shift = p * bits, from = (p + 1) & 1, to = p & 1;
+    const bool last = p + 1 == digits;
+    int rc = dispatch_id(id_type, [&](auto id) {
+      using Id = decltype(id);
+      const RowKeys<Id> rows{p == 0 ? (const Id*)d_ids : nullptr, plan->d_keys[from], plan->d_vals[from], (uint32_t)ids};
+      hipLaunchKernelGGL((digit_count_kernel<Id>), dim3((unsigned)tiles), dim3(kDigitThreads), 0, st, n, rows, shift, bits,
+                         tiles, fused ? 0 : 1, plan->d_hist);
+      if (!fused)
+        if (int e = exclusive_scan_u32(plan->d_hist, plan->d_hist, tiles << bits, st, plan->d_scan)) return e;
+      hipLaunchKernelGGL((digit_scatter_kernel<Id>), dim3((unsigned)tiles), dim3(kDigitThreads), 0, st, n, rows, shift, bits,
+                         tiles, fused ? 0 : 1, plan->d_hist, last && d_order && with_offsets ? nullptr : plan->d_keys[to],
+                         last && d_order ? d_order : plan->d_vals[to], ids, with_offsets ? d_offsets : nullptr);
+      return (int)HPSPMM_OK;
+    });
+    if (rc) return rc;
+  }
+  const int at = (digits - 1) & 1;
+  if (d_offsets && !with_offsets)
+    hipLaunchKernelGGL(row_offsets_kernel, dim3((unsigned)ceil_div(n_offsets, kBlock)), dim3(kBlock), 0, st, n, ids,
+                       plan->d_keys[at], d_offsets);
+  if (out) *out = {plan->d_keys[at], plan->d_vals[at]};
+  return HPSPMM_OK;
+}
+
+// Shape of the sums of a gradient with rows of `width` columns, `per16` of which a thread owns.
+struct SumShape {
+  int tpr_log2, chunk_log2;
+  int64_t col_tiles, chunks, pitch;
+};
+constexpr int kMinChunkLog2 = 3, kMaxChunkLog2 = 7;
+SumShape sum_shape(int64_t n, int64_t width, int64_t per16) {
+  SumShape s{};
+  const int64_t vecs = ceil_div(width, per16);
+  while (s.tpr_log2 < 8 && ((int64_t)1 << s.tpr_log2) < vecs) ++s.tpr_log2;
+  s.col_tiles = ceil_div(vecs, (int64_t)1 << s.tpr_log2);
+  // chunks as long as leaves 2048 of them a column tile, at most 128 rows
+  s.chunk_log2 = kMinChunkLog2;
+  while (s.chunk_log2 < kMaxChunkLog2 && (n * s.col_tiles) >> (s.chunk_log2 + 1) >= 2048) ++s.chunk_log2;
+  s.chunks = ceil_div(n, (int64_t)1 << s.chunk_log2);
+  s.pitch = ceil_div(width, 8) * 8;
+  return s;
+}
+// Carry floats that any n <= rows, width <= columns can need.
+int64_t most_carry_floats(int64_t rows, int64_t columns) {
+  if (rows == 0 || columns == 0) return 0;
+  // a column tile has at most 2048 columns; chunks * tiles stays below 4096 (+ one chunk) until chunks are at their longest
+  const int64_t tiles = ceil_div(columns, 4 * hpspmm::kBlock), pitch = ceil_div(columns, 8) * 8;
+  const int64_t by_rows = 2 * ceil_div(rows, (int64_t)1 << kMinChunkLog2) * pitch;
+  const int64_t by_tiles = 2 * 2048 * (std::max<int64_t>(4096, (rows * tiles) >> kMaxChunkLog2) + tiles + 1);
+  return std::min(by_rows, by_tiles);
 }
 
 }  // namespace
@@ -85,9 +161,13 @@ HPSPMM_API int hpspmm_rows_plan_create(int64_t max_rows, int64_t max_ids, int64_
   p->max_rows = max_rows;
   p->max_ids = max_ids;
   p->max_width = max_width;
-  const int64_t n = std::max<int64_t>(max_rows, 1), tiles = ceil_div(n, sort_tile());
-  const int64_t hist = 256 * tiles + 1, scan = scan_scratch_words(256 * tiles);
-  const int64_t words[] = {n, n, n, n, hist, scan};
+  int digits, bits;
+  key_digits(max_ids, &digits, &bits);
+  const int64_t n = std::max<int64_t>(max_rows, 1), tiles = ceil_div(n, hpspmm::kDigitTile);
+  // (fewer ids may make a digit of more bits)
+  const int64_t hist = tiles << std::min<int>(hpspmm::kDigitBits, key_bits(max_ids)), scan = scan_scratch_words(hist);
+  const int64_t carry = most_carry_floats(max_rows, max_width);
+  const int64_t words[] = {n, n, n, n, hist, scan, carry};
   int64_t bytes = 0;
   for (int64_t w : words) bytes += (w * 4 + 255) & ~(int64_t)255;
   if (hipMalloc((void**)&p->arena, (size_t)bytes) != hipSuccess) {
@@ -108,6 +188,8 @@ HPSPMM_API int hpspmm_rows_plan_create(int64_t max_rows, int64_t max_ids, int64_
   p->d_vals[1] = (int32_t*)take(n);
   p->d_hist = (uint32_t*)take(hist);
   p->d_scan = (uint32_t*)take(scan);
+  p->d_carry = (float*)take(carry);
+  p->carry_floats = carry;
   *plan_out = p;
   return HPSPMM_OK;
 }
@@ -137,14 +219,19 @@ HPSPMM_API int hpspmm_embedding_lookup(int64_t n, int64_t vocab, int64_t width, 
   const int64_t col_tiles = ceil_div(vecs, (int64_t)1 << tpr_log2);
   const int64_t per_pass = hpspmm::kBlock >> tpr_log2;
   const bool many = n * col_tiles >= 4 * per_pass * 1024;
-  const int64_t blocks = ceil_div(n, per_pass * (many ? 4 : 1));
+  // (a launch holds fewer than 2^32 threads: 2^23 workgroups at a time)
+  const int64_t per_block = per_pass * (many ? 4 : 1), per_launch = per_block << 23;
   dispatch_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     return dispatch_id(id_type, [&](auto id) {
       using Id = decltype(id);
       auto launch = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, (unsigned)col_tiles), dim3(hpspmm::kBlock), 0, st, n, (uint32_t)vocab,
-                           (int32_t)width, tpr_log2, (const Id*)d_ids, (const T*)d_table, ld_table, scale, (T*)d_out, ld_out);
+        for (int64_t r = 0; r < n; r += per_launch) {
+          const int64_t rows = std::min(per_launch, n - r);
+          hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(rows, per_block), (unsigned)col_tiles), dim3(hpspmm::kBlock), 0, st,
+                             rows, (uint32_t)vocab, (int32_t)width, tpr_log2, (const Id*)d_ids + r, (const T*)d_table, ld_table,
+                             scale, (T*)d_out + r * ld_out, ld_out);
+        }
       };
       if (aligned) {
         if (many) launch(hpspmm::embedding_lookup_kernel<T, Id, true, 4>);
@@ -167,11 +254,7 @@ HPSPMM_API int hpspmm_group_rows(hpspmm_rows_plan* plan, int64_t n, int64_t grou
   if (!aligned_to(d_order, 4) || !aligned_to(d_offsets, 4))
     return fail(HPSPMM_ERR_INVALID_ARG, "d_order or d_offsets is not at a multiple of 4 bytes");
   if (int rc = check_rows_plan(plan, n, groups, 0)) return rc;
-  hipStream_t st = (hipStream_t)stream;
-  int cur = 0;
-  if (int rc = sort_rows(plan, n, groups, d_ids, id_type, st, &cur)) return rc;
-  hipLaunchKernelGGL(hpspmm::row_offsets_kernel, dim3((unsigned)ceil_div(std::max(n, groups + 1), hpspmm::kBlock)),
-                     dim3(hpspmm::kBlock), 0, st, n, groups, plan->d_keys[cur], plan->d_vals[cur], d_order, d_offsets);
+  if (int rc = sort_rows(plan, n, groups, d_ids, id_type, d_order, d_offsets, (hipStream_t)stream, nullptr)) return rc;
   HPSPMM_HIP(hipGetLastError());
   return HPSPMM_OK;
 }
@@ -187,18 +270,41 @@ HPSPMM_API int hpspmm_embedding_grad(hpspmm_rows_plan* plan, int64_t n, int64_t 
   if (int rc = check_rows_plan(plan, n, vocab, width)) return rc;
   if (vocab == 0 || (n == 0 && accumulate)) return HPSPMM_OK;
   hipStream_t st = (hipStream_t)stream;
-  int cur = 0;
-  if (int rc = sort_rows(plan, n, vocab, d_ids, id_type, st, &cur)) return rc;
-  dispatch_dtype(grad_type, [&](auto t) {
-    using T = decltype(t);
-    return dispatch_dtype(table_type, [&](auto o) {
-      using TO = decltype(o);
-      hipLaunchKernelGGL((hpspmm::embedding_grad_kernel<T, TO>),
-                         dim3((unsigned)vocab, (unsigned)std::min<int64_t>(ceil_div(width, hpspmm::kBlock), 64)),
-                         dim3(hpspmm::kBlock), 0, st, n, (int32_t)width, plan->d_keys[cur], plan->d_vals[cur],
-                         (const T*)d_grad, ld_grad, scale, (TO*)d_table, ld_table, accumulate);
+  Sorted sorted{};
+  if (int rc = sort_rows(plan, n, vocab, d_ids, id_type, nullptr, nullptr, st, &sorted)) return rc;
+  const int64_t grad_size = dtype_size(grad_type), table_size = dtype_size(table_type);
+  const SumShape s = sum_shape(n, width, 16 / grad_size);
+  if (2 * s.chunks * s.pitch > plan->carry_floats) return fail(HPSPMM_ERR_INVALID_ARG, "the plan's workspace is too small");
+  const int64_t per_block = s.tpr_log2 < 6 ? hpspmm::kBlock >> s.tpr_log2 : 1;
+  const int64_t sum_blocks = ceil_div(s.chunks, per_block);
+  const int64_t zero_blocks = accumulate ? 0 : std::min<int64_t>(ceil_div(vocab, hpspmm::kZeroRows), 1 << 20);
+  const unsigned threads = s.tpr_log2 < 6 ? hpspmm::kBlock : 1u << s.tpr_log2;
+  const bool aligned = aligned_to(d_grad, 16) && aligned_to(d_table, 16) && ld_grad * grad_size % 16 == 0 && ld_table * table_size % 16 == 0;
+  const hpspmm::SumArgs g{n, (uint32_t)vocab, (int32_t)width, (int32_t)s.pitch, sorted.keys, sorted.rows, d_grad, ld_grad, scale,
+                          d_table, ld_table, accumulate != 0, plan->d_carry, s.chunk_log2, s.tpr_log2, s.chunks, (unsigned)sum_blocks,
+                          (unsigned)zero_blocks};
+  const dim3 fix_grid((unsigned)ceil_div(s.chunks, hpspmm::kFixChunks), (unsigned)ceil_div(width, 256));
+  dispatch_dtype(table_type, [&](auto o) {
+    using TO = decltype(o);
+    dispatch_dtype(grad_type, [&](auto t) {
+      using T = decltype(t);
+      auto launch = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(sum_blocks + zero_blocks), (unsigned)s.col_tiles), dim3(threads), 0, st, g);
+      };
+      if (s.tpr_log2 >= 6) {
+        if (aligned) launch(hpspmm::embedding_sum_kernel<T, TO, true, true>);
+        else launch(hpspmm::embedding_sum_kernel<T, TO, false, true>);
+      } else {
+        if (aligned) launch(hpspmm::embedding_sum_kernel<T, TO, true, false>);
+        else launch(hpspmm::embedding_sum_kernel<T, TO, false, false>);
+      }
       return HPSPMM_OK;
     });
+    if (s.chunks > 1) {
+      if (aligned) hipLaunchKernelGGL((hpspmm::embedding_fix_kernel<TO, true>), fix_grid, dim3(hpspmm::kBlock), 0, st, g);
+      else hipLaunchKernelGGL((hpspmm::embedding_fix_kernel<TO, false>), fix_grid, dim3(hpspmm::kBlock), 0, st, g);
+    }
+    return HPSPMM_OK;
   });
   HPSPMM_HIP(hipGetLastError());
   return HPSPMM_OK;

@@ -12,8 +12,10 @@ struct hpspmm_rows_plan {
   int64_t workspace_bytes = 0;
   uint32_t* d_keys[2] = {nullptr, nullptr};  // [max_rows] ids, sorted
   int32_t* d_vals[2] = {nullptr, nullptr};   // [max_rows] the rows they belong to
-  uint32_t* d_hist = nullptr;
+  uint32_t* d_hist = nullptr;                // [tiles * bins] counts per digit and tile of rows
   uint32_t* d_scan = nullptr;
+  float* d_carry = nullptr;                  // sums that cross chunks of the sorted rows
+  int64_t carry_floats = 0;
 };
 
 namespace hpspmm_host {
