@@ -55,6 +55,50 @@ __global__ __launch_bounds__(kBlock) void embedding_lookup_kernel(int64_t n, uin
   }
 }
 
+// Rows of zeros, for the launches that have workgroups to spare: rows [0, rows) of `bytes` + `tail` bytes each, `pitch`
+// bytes apart, by `blocks` workgroups from workgroup `first` on.  An all-zero word is a zero of every element type.
+struct ZeroFill {
+  char* at;
+  int64_t rows, bytes, pitch;
+  unsigned first, blocks;
+  int unit, tail;  // bytes of a store: 16, 4 or 2 (address, `bytes` and pitch are multiples of it); what is left, 0 ... 14
+};
+template <class U>
+__device__ __forceinline__ void fill_units(const ZeroFill& z) {
+  const int64_t rows = z.rows;
+  const int64_t units = z.bytes / (int64_t)sizeof(U);
+  const U zero{};
+  if (units >= (int64_t)blockDim.x * 4) {
+    // whole workgroups along a row, 4 stores a thread and step
+    const int64_t pieces = (units + 4 * (int64_t)blockDim.x - 1) / (4 * (int64_t)blockDim.x);
+    for (int64_t p = (int64_t)blockIdx.x - z.first; p < rows * pieces; p += z.blocks) {
+      const int64_t r = p / pieces, u0 = (p - r * pieces) * 4 * blockDim.x + threadIdx.x;
+      U* row = (U*)(z.at + r * z.pitch);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t u = u0 + q * (int64_t)blockDim.x;
+        if (u < units) row[u] = zero;
+      }
+    }
+  } else {
+    const int64_t all = rows * units;  // (none where a row is shorter than a store)
+    for (int64_t i = ((int64_t)blockIdx.x - z.first) * blockDim.x + threadIdx.x; i < all; i += (int64_t)z.blocks * blockDim.x) {
+      const int64_t r = i / units;
+      ((U*)(z.at + r * z.pitch))[i - r * units] = zero;
+    }
+  }
+}
+__device__ __forceinline__ void zero_fill(const ZeroFill& z) {
+  if (z.unit == 16) fill_units<uint4>(z);
+  else if (z.unit == 4) fill_units<uint32_t>(z);
+  else fill_units<uint16_t>(z);
+  const int64_t left = z.rows * (z.tail / 2);
+  for (int64_t i = ((int64_t)blockIdx.x - z.first) * blockDim.x + threadIdx.x; i < left; i += (int64_t)z.blocks * blockDim.x) {
+    const int64_t r = i / (z.tail / 2);
+    ((uint16_t*)(z.at + r * z.pitch + z.bytes))[i - r * (z.tail / 2)] = 0;
+  }
+}
+
 // ---------------------------------------------------------------------------------------------
 // Rows sorted by id: keys[q] / vals[q] = id and row of the q-th row in that order, rows of one id in increasing order,
 // ids outside [0, ids) as key `ids` behind all others.
@@ -88,7 +132,8 @@ template <class Id>
 __global__ __launch_bounds__(64 * kRankWaves) void row_rank_kernel(int32_t n, int32_t n_virtual, uint32_t ids,
                                                                   const Id* __restrict__ id, uint32_t* __restrict__ keys,
                                                                   int32_t* __restrict__ vals,
-                                                                  int32_t* __restrict__ offsets) {
+                                                                  int32_t* __restrict__ offsets, ZeroFill zero) {
+  if (blockIdx.x >= zero.first) return zero_fill(zero);
   __shared__ __attribute__((aligned(16))) uint32_t s_key[kRankMaxRows];
   __shared__ int32_t s_count[kRankWaves][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -149,7 +194,7 @@ __global__ __launch_bounds__(64 * kRankWaves) void row_rank_kernel(int32_t n, in
 // tile of rows, then the rows to their places.  A tile's rows go to the wavefronts in stretches of 4 x 64; a row's rank
 // among the equal digits of its stretch is found by ballots over the digit's bits.
 constexpr int kDigitBits = 10, kDigitBins = 1 << kDigitBits;
-constexpr int kDigitThreads = 512, kDigitWaves = kDigitThreads / 64, kDigitRounds = 4;
+constexpr int kDigitThreads = 1024, kDigitWaves = kDigitThreads / 64, kDigitRounds = 4;
 constexpr int kDigitTile = kDigitThreads * kDigitRounds;
 constexpr int kDigitFused = 256;  // up to so many tiles every workgroup adds up the counts of the others itself
 
@@ -167,7 +212,9 @@ struct RowKeys {
 // hist[tile * bins + d] (or hist[d * tiles + tile], for a scan over all of it) = rows of the tile with digit d.
 template <class Id>
 __global__ __launch_bounds__(kDigitThreads) void digit_count_kernel(int64_t n, RowKeys<Id> rows, int shift, int bits,
-                                                                   int64_t tiles, int by_digit, uint32_t* __restrict__ hist) {
+                                                                   int64_t tiles, int by_digit, uint32_t* __restrict__ hist,
+                                                                   ZeroFill zero) {
+  if (blockIdx.x >= zero.first) return zero_fill(zero);
   __shared__ uint32_t s_hist[kDigitBins];
   const int bins = 1 << bits;
   for (int d = threadIdx.x; d < bins; d += kDigitThreads) s_hist[d] = 0;
@@ -192,9 +239,11 @@ __global__ __launch_bounds__(kDigitThreads) void digit_scatter_kernel(int64_t n,
                                                                      const uint32_t* __restrict__ hist,
                                                                      uint32_t* __restrict__ keys_out,
                                                                      int32_t* __restrict__ vals_out, int64_t groups,
-                                                                     int32_t* __restrict__ offsets) {
+                                                                     int32_t* __restrict__ offsets, ZeroFill zero) {
+  if (blockIdx.x >= zero.first) return zero_fill(zero);
   __shared__ uint32_t s_base[kDigitBins];
   __shared__ uint32_t s_wave[kDigitWaves][kDigitBins];
+  __shared__ uint32_t s_part[2][kDigitThreads];
   __shared__ uint32_t s_sum[kDigitWaves];
   const int bins = 1 << bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t tile = blockIdx.x, base = tile * kDigitTile;
@@ -229,21 +278,28 @@ __global__ __launch_bounds__(kDigitThreads) void digit_scatter_kernel(int64_t n,
   if (scanned) {
     for (int d = threadIdx.x; d < bins; d += kDigitThreads) s_base[d] = hist[(int64_t)d * tiles + tile];
   } else {
-    // (two bins a thread at most)
-    uint32_t all[2] = {0, 0}, earlier[2] = {0, 0};
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int d = (int)threadIdx.x * 2 + h;
-      if (d < bins) {
-#pragma unroll 8
-        for (int64_t t = 0; t < tiles; ++t) {
-          const uint32_t c = hist[t * bins + d];
-          all[h] += c;
-          if (t < tile) earlier[h] += c;
-        }
-      }
+    // kDigitThreads / bins threads share a bin, each adds up a stretch of the tiles; their sums meet in s_part
+    const int d = threadIdx.x & (bins - 1), share = (int)threadIdx.x >> bits, shares = kDigitThreads >> bits;
+    const int64_t per = (tiles + shares - 1) / shares, first = share * per, stop = min(first + per, tiles);
+    uint32_t all = 0, earlier = 0;
+#pragma unroll 16
+    for (int64_t t = first; t < stop; ++t) {
+      const uint32_t c = hist[t * bins + d];
+      all += c;
+      if (t < tile) earlier += c;
     }
-    uint32_t upto = all[0] + all[1];
+    s_part[0][threadIdx.x] = all;
+    s_part[1][threadIdx.x] = earlier;
+    __syncthreads();
+    if (share == 0) {
+      for (int h = 1; h < shares; ++h) {
+        all += s_part[0][(h << bits) + d];
+        earlier += s_part[1][(h << bits) + d];
+      }
+    } else {
+      all = 0;
+    }
+    uint32_t upto = all;
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
       const uint32_t other = __shfl_up(upto, s, 64);
@@ -251,16 +307,11 @@ __global__ __launch_bounds__(kDigitThreads) void digit_scatter_kernel(int64_t n,
     }
     if (lane == 63) s_sum[wave] = upto;
     __syncthreads();
-    uint32_t start = upto - all[0] - all[1];
+    uint32_t start = upto - all;
     for (int w = 0; w < wave; ++w) start += s_sum[w];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int d = (int)threadIdx.x * 2 + h;
-      if (d < bins) {
-        s_base[d] = start + earlier[h];
-        if (offsets && tile == 0 && d <= groups) offsets[d] = (int32_t)start;
-      }
-      start += all[h];
+    if (share == 0) {
+      s_base[d] = start + earlier;
+      if (offsets && tile == 0 && d <= groups) offsets[d] = (int32_t)start;
     }
   }
   __syncthreads();
@@ -293,33 +344,38 @@ __global__ __launch_bounds__(kDigitThreads) void digit_scatter_kernel(int64_t n,
 
 constexpr int kSumFlight = 8;  // rows in flight
 
-template <class T, bool kAligned>
+// kWhole: rows at multiples of 16 bytes whose 16-byte pieces are all whole; otherwise any alignment and length.
+template <class T, bool kWhole>
 __device__ __forceinline__ void load_row(const T* p, int there, float (&v)[kPer16<T>]) {
-  if (there >= kPer16<T>) {
-    load16<kAligned>(p, v);
+  if (kWhole || there >= kPer16<T>) {
+    load16<kWhole>(p, v);
   } else {
 #pragma unroll
     for (int i = 0; i < kPer16<T>; ++i) v[i] = i < there ? (float)p[i] : 0.f;
   }
 }
 
+// Sorted keys and rows, as the kernel finds them: reads at addresses that a whole workgroup shares go through scalar
+// registers.
+template <class T>
+using Fixed = const __attribute__((address_space(4))) T*;
+
 // at[0 .. there) = (accumulate ? at : 0) + scale * v.
-template <class TO, int kN, bool kAligned>
+template <class TO, int kN, bool kWhole>
 __device__ __forceinline__ void store_sum(TO* at, int there, const float (&v)[kN], float scale, int accumulate) {
   constexpr int kPart = kN < kPer16<TO> ? kN : kPer16<TO>;
 #pragma unroll
   for (int p = 0; p < kN; p += kPart) {
     float out[kPart];
-    if (there >= p + kPart) {
+    if (kWhole || there >= p + kPart) {
+#pragma unroll
+      for (int i = 0; i < kPart; ++i) out[i] = scale * v[p + i];
       if (accumulate) {
-        const auto old = *reinterpret_cast<const typename Pack<TO, kPart, kAligned>::type*>(at + p);
+        const auto old = *reinterpret_cast<const typename Pack<TO, kPart, kWhole>::type*>(at + p);
 #pragma unroll
-        for (int i = 0; i < kPart; ++i) out[i] = (float)old[i] + scale * v[p + i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < kPart; ++i) out[i] = scale * v[p + i];
+        for (int i = 0; i < kPart; ++i) out[i] += (float)old[i];
       }
-      store_n<kAligned, TO, kPart>(at + p, out);
+      store_n<kWhole, TO, kPart>(at + p, out);
     } else {
 #pragma unroll
       for (int i = 0; i < kPart; ++i)
@@ -349,7 +405,7 @@ struct SumArgs {
 
 constexpr int kZeroRows = 64;  // rows of the table a workgroup looks at for that
 
-template <class T, class TO, bool kAligned, bool kWide>
+template <class T, class TO, bool kWhole, bool kWide>
 __global__ __launch_bounds__(kBlock) void embedding_sum_kernel(SumArgs g) {
   constexpr int V = kPer16<T>;
   const int tpr = 1 << g.tpr_log2;
@@ -371,7 +427,7 @@ __global__ __launch_bounds__(kBlock) void embedding_sum_kernel(SumArgs g) {
         rows &= rows - 1;
         TO* row = (TO*)g.d_table + (v0 + r) * g.ld_table;
         for (int c = (int)threadIdx.x * kPart; c < g.width; c += (int)blockDim.x * kPart)
-          store_sum<TO, kPart, kAligned>(row + c, g.width - c, zero, 0.f, 0);
+          store_sum<TO, kPart, false>(row + c, g.width - c, zero, 0.f, 0);
       }
     }
     return;
@@ -381,9 +437,11 @@ __global__ __launch_bounds__(kBlock) void embedding_sum_kernel(SumArgs g) {
   const int there = g.width - col;
   if (c >= g.chunks || there <= 0) return;
   const int64_t begin = c << g.chunk_log2, end = min(begin + ((int64_t)1 << g.chunk_log2), g.n);
-  uint32_t cur = g.keys[begin];
+  const Fixed<uint32_t> keys = (Fixed<uint32_t>)(uintptr_t)g.keys;
+  const Fixed<int32_t> pos = (Fixed<int32_t>)(uintptr_t)g.pos;
+  uint32_t cur = keys[begin];
   if (cur >= g.vocab) return;
-  bool open = begin > 0 && g.keys[begin - 1] == cur;  // the sum began in an earlier chunk
+  bool open = begin > 0 && keys[begin - 1] == cur;  // the sum began in an earlier chunk
   float acc[V] = {};
   const T* grad = (const T*)g.grad + col;
   auto close = [&](int slot) {
@@ -391,7 +449,7 @@ __global__ __launch_bounds__(kBlock) void embedding_sum_kernel(SumArgs g) {
       float* at = g.carry + (2 * c + slot) * (int64_t)g.pitch + col;
       store_sum<float, V, true>(at, g.pitch - col, acc, 1.f, 0);
     } else {
-      store_sum<TO, V, kAligned>((TO*)g.d_table + (int64_t)cur * g.ld_table + col, there, acc, g.scale, g.accumulate);
+      store_sum<TO, V, kWhole>((TO*)g.d_table + (int64_t)cur * g.ld_table + col, there, acc, g.scale, g.accumulate);
     }
   };
   bool done = false;
@@ -400,8 +458,8 @@ __global__ __launch_bounds__(kBlock) void embedding_sum_kernel(SumArgs g) {
     float row[kSumFlight][V];
 #pragma unroll
     for (int u = 0; u < kSumFlight; ++u) {
-      key[u] = q0 + u < end ? g.keys[q0 + u] : g.vocab;
-      if (key[u] < g.vocab) load_row<T, kAligned>(grad + (int64_t)g.pos[q0 + u] * g.ld_grad, there, row[u]);
+      key[u] = q0 + u < end ? keys[q0 + u] : g.vocab;
+      if (key[u] < g.vocab) load_row<T, kWhole>(grad + (int64_t)pos[q0 + u] * g.ld_grad, there, row[u]);
     }
 #pragma unroll
     for (int u = 0; u < kSumFlight; ++u) {
@@ -427,52 +485,53 @@ __global__ __launch_bounds__(kBlock) void embedding_sum_kernel(SumArgs g) {
     }
   }
   if (cur >= g.vocab) return;
-  const bool goes_on = end < g.n && g.keys[end] == cur;
+  const bool goes_on = end < g.n && keys[end] == cur;
   close(open ? 0 : goes_on ? 1 : -1);
 }
 
-// The sums that cross chunks: the chunk in which one begins adds up its slots.  A workgroup looks at kFixChunks chunks
-// and owns 256 columns; its wavefronts take a stretch of the slots each, and their sums are added in that order.
-constexpr int kFixChunks = 8;
-template <class TO, bool kAligned>
+// The sums that cross chunks: the chunk in which one begins adds up its slots.  One workgroup per chunk and 256 columns;
+// its wavefronts take a stretch of the slots each, and their sums are added in that order.
+template <class TO, bool kWhole>
 __global__ __launch_bounds__(kBlock) void embedding_fix_kernel(SumArgs g) {
   __shared__ float s_part[kWavesPerBlock][64][4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int col = ((int)blockIdx.y * 64 + lane) * 4, there = g.width - col;
-  for (int64_t c = (int64_t)blockIdx.x * kFixChunks; c < min((int64_t)(blockIdx.x + 1) * kFixChunks, g.chunks); ++c) {
-    const int64_t begin = c << g.chunk_log2, end = min(begin + ((int64_t)1 << g.chunk_log2), g.n);
-    if (end >= g.n) return;
-    const uint32_t key = g.keys[end - 1];
-    if (key >= g.vocab) return;
-    if (g.keys[end] != key) continue;                                                // it ends here
-    if (g.keys[begin] == key && begin > 0 && g.keys[begin - 1] == key) continue;     // it began earlier
-    const int64_t stop = lower_bound_u32(g.keys, g.n, key + 1);
-    const int64_t slots = ((stop - 1) >> g.chunk_log2) - c;  // chunks behind this one that it reaches
-    const int64_t per = (slots + kWavesPerBlock - 1) / kWavesPerBlock;
-    const int64_t first = wave * per, last = min(first + per, slots);
-    float acc[4] = {};
-    if (there > 0) {
-      if (wave == 0) load16<true>(g.carry + (2 * c + 1) * (int64_t)g.pitch + col, acc);
-#pragma unroll 8
-      for (int64_t s = first; s < last; ++s) {
-        float v[4];
-        load16<true>(g.carry + 2 * (c + 1 + s) * (int64_t)g.pitch + col, v);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] += v[i];
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s_part[wave][lane][i] = acc[i];
-    __syncthreads();
-    if (wave == 0 && there > 0) {
-#pragma unroll
-      for (int w = 1; w < kWavesPerBlock; ++w)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] += s_part[w][lane][i];
-      store_sum<TO, 4, kAligned>((TO*)g.d_table + (int64_t)key * g.ld_table + col, there, acc, g.scale, g.accumulate);
-    }
-    __syncthreads();
+  const int64_t c = blockIdx.x, begin = c << g.chunk_log2, end = begin + ((int64_t)1 << g.chunk_log2);
+  if (end >= g.n) return;
+  const uint32_t key = g.keys[end - 1], next = g.keys[end], first_key = g.keys[begin], before = g.keys[begin > 0 ? begin - 1 : 0];
+  if (key >= g.vocab || next != key) return;                     // it ends here
+  if (begin > 0 && first_key == key && before == key) return;    // it began earlier
+  // chunks behind this one that begin within the sum, 64 a step
+  int64_t slots = 0;
+  for (;;) {
+    const int64_t at = (c + 1 + slots + lane) << g.chunk_log2;
+    const uint64_t within = __ballot(at < g.n && g.keys[min(at, g.n - 1)] == key);
+    const int more = __popcll(within);
+    slots += more;
+    if (more < 64) break;
   }
+  const int col = ((int)blockIdx.y * 64 + lane) * 4, there = g.width - col;
+  const int64_t per = (slots + kWavesPerBlock - 1) / kWavesPerBlock;
+  const int64_t first = wave * per, last = min(first + per, slots);
+  float acc[4] = {};
+  if (there > 0) {
+    if (wave == 0) load16<true>(g.carry + (2 * c + 1) * (int64_t)g.pitch + col, acc);
+#pragma unroll 8
+    for (int64_t s = first; s < last; ++s) {
+      float v[4];
+      load16<true>(g.carry + 2 * (c + 1 + s) * (int64_t)g.pitch + col, v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] += v[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s_part[wave][lane][i] = acc[i];
+  __syncthreads();
+  if (wave != 0 || there <= 0) return;
+#pragma unroll
+  for (int w = 1; w < kWavesPerBlock; ++w)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] += s_part[w][lane][i];
+  store_sum<TO, 4, kWhole>((TO*)g.d_table + (int64_t)key * g.ld_table + col, there, acc, g.scale, g.accumulate);
 }
 
 }  // namespace hpspmm

@@ -68,21 +68,51 @@ struct Sorted {
   const uint32_t* keys;
   const int32_t* rows;
 };
+// The rows of a table that become zeros, cut into stretches for launches to come.
+struct ZeroRows {
+  char* at = nullptr;
+  int64_t rows = 0, bytes = 0, pitch = 0;
+  bool flat = false;  // one stretch of memory, rows * bytes long
+  // The next of `left` stretches, for a launch of `first` workgroups of `threads` threads; *grid = the workgroups in all.
+  hpspmm::ZeroFill next(int64_t first, int left, int threads, unsigned* grid) {
+    hpspmm::ZeroFill z{at, 0, bytes, pitch, (unsigned)first, 0, 16, 0};
+    const int64_t share = ceil_div(rows, left);
+    if (flat) {
+      z.rows = share > 0;
+      z.bytes = share * bytes;
+      z.pitch = 0;
+    } else {
+      z.rows = share;
+    }
+    at += share * pitch;
+    rows -= share;
+    const int64_t apart = (int64_t)(uintptr_t)z.at | z.pitch;
+    z.unit = apart % 16 == 0 ? 16 : apart % 4 == 0 ? 4 : 2;
+    z.tail = (int)(z.bytes % z.unit);
+    z.bytes -= z.tail;
+    z.blocks = (unsigned)std::min<int64_t>(ceil_div(z.rows * (z.bytes + z.tail), (int64_t)z.unit * threads * 4), 4096);
+    *grid = (unsigned)first + z.blocks;
+    return z;
+  }
+};
+
 int sort_rows(hpspmm_rows_plan* plan, int64_t n, int64_t ids, const void* d_ids, int id_type, int32_t* d_order,
-              int32_t* d_offsets, hipStream_t st, Sorted* out) {
+              int32_t* d_offsets, ZeroRows zero, hipStream_t st, Sorted* out) {
   using namespace hpspmm;
+  unsigned grid = 0;
   if (out) *out = {plan->d_keys[0], plan->d_vals[0]};
   const int64_t n_offsets = d_offsets ? ids + 1 : 0;
   // Counting ranks costs n^2 / 16 steps of a wavefront in all, digits two dependent launches each: 512 rows 5 us against
   // 12, 8192 rows and 2^17 ids 10 against 20, about the same at 16384.
   if (n <= kRankMaxRows && (n_offsets <= 4 * kRankMaxRows || n == 0)) {
     const int64_t count = n + n_offsets;
-    if (count == 0) return HPSPMM_OK;
+    if (count == 0 && zero.rows == 0) return HPSPMM_OK;
+    const ZeroFill z = zero.next(ceil_div(count, 64), 1, 64 * kRankWaves, &grid);
     return dispatch_id(id_type, [&](auto id) {
       using Id = decltype(id);
-      hipLaunchKernelGGL((row_rank_kernel<Id>), dim3((unsigned)ceil_div(count, 64)), dim3(64 * kRankWaves), 0, st, (int32_t)n,
+      hipLaunchKernelGGL((row_rank_kernel<Id>), dim3(grid), dim3(64 * kRankWaves), 0, st, (int32_t)n,
                          (int32_t)n_offsets, (uint32_t)ids, (const Id*)d_ids, d_order ? nullptr : plan->d_keys[0],
-                         d_order ? d_order : plan->d_vals[0], d_offsets);
+                         d_order ? d_order : plan->d_vals[0], d_offsets, z);
       return HPSPMM_OK;
     });
   }
@@ -98,13 +128,15 @@ int sort_rows(hpspmm_rows_plan* plan, int64_t n, int64_t ids, const void* d_ids,
     int rc = dispatch_id(id_type, [&](auto id) {
       using Id = decltype(id);
       const RowKeys<Id> rows{p == 0 ? (const Id*)d_ids : nullptr, plan->d_keys[from], plan->d_vals[from], (uint32_t)ids};
-      hipLaunchKernelGGL((digit_count_kernel<Id>), dim3((unsigned)tiles), dim3(kDigitThreads), 0, st, n, rows, shift, bits,
-                         tiles, fused ? 0 : 1, plan->d_hist);
+      ZeroFill z = zero.next(tiles, 2 * (digits - p), kDigitThreads, &grid);
+      hipLaunchKernelGGL((digit_count_kernel<Id>), dim3(grid), dim3(kDigitThreads), 0, st, n, rows, shift, bits,
+                         tiles, fused ? 0 : 1, plan->d_hist, z);
       if (!fused)
         if (int e = exclusive_scan_u32(plan->d_hist, plan->d_hist, tiles << bits, st, plan->d_scan)) return e;
-      hipLaunchKernelGGL((digit_scatter_kernel<Id>), dim3((unsigned)tiles), dim3(kDigitThreads), 0, st, n, rows, shift, bits,
+      z = zero.next(tiles, 2 * (digits - p) - 1, kDigitThreads, &grid);
+      hipLaunchKernelGGL((digit_scatter_kernel<Id>), dim3(grid), dim3(kDigitThreads), 0, st, n, rows, shift, bits,
                          tiles, fused ? 0 : 1, plan->d_hist, last && d_order && with_offsets ? nullptr : plan->d_keys[to],
-                         last && d_order ? d_order : plan->d_vals[to], ids, with_offsets ? d_offsets : nullptr);
+                         last && d_order ? d_order : plan->d_vals[to], ids, with_offsets ? d_offsets : nullptr, z);
       return (int)HPSPMM_OK;
     });
     if (rc) return rc;
@@ -128,9 +160,9 @@ SumShape sum_shape(int64_t n, int64_t width, int64_t per16) {
   const int64_t vecs = ceil_div(width, per16);
   while (s.tpr_log2 < 8 && ((int64_t)1 << s.tpr_log2) < vecs) ++s.tpr_log2;
   s.col_tiles = ceil_div(vecs, (int64_t)1 << s.tpr_log2);
-  // chunks as long as leaves 2048 of them a column tile, at most 128 rows
+  // chunks as long as leaves 1024 of them a column tile, at most 128 rows
   s.chunk_log2 = kMinChunkLog2;
-  while (s.chunk_log2 < kMaxChunkLog2 && (n * s.col_tiles) >> (s.chunk_log2 + 1) >= 2048) ++s.chunk_log2;
+  while (s.chunk_log2 < kMaxChunkLog2 && (n * s.col_tiles) >> (s.chunk_log2 + 1) >= 1024) ++s.chunk_log2;
   s.chunks = ceil_div(n, (int64_t)1 << s.chunk_log2);
   s.pitch = ceil_div(width, 8) * 8;
   return s;
@@ -254,7 +286,7 @@ HPSPMM_API int hpspmm_group_rows(hpspmm_rows_plan* plan, int64_t n, int64_t grou
   if (!aligned_to(d_order, 4) || !aligned_to(d_offsets, 4))
     return fail(HPSPMM_ERR_INVALID_ARG, "d_order or d_offsets is not at a multiple of 4 bytes");
   if (int rc = check_rows_plan(plan, n, groups, 0)) return rc;
-  if (int rc = sort_rows(plan, n, groups, d_ids, id_type, d_order, d_offsets, (hipStream_t)stream, nullptr)) return rc;
+  if (int rc = sort_rows(plan, n, groups, d_ids, id_type, d_order, d_offsets, ZeroRows{}, (hipStream_t)stream, nullptr)) return rc;
   HPSPMM_HIP(hipGetLastError());
   return HPSPMM_OK;
 }
@@ -270,20 +302,33 @@ HPSPMM_API int hpspmm_embedding_grad(hpspmm_rows_plan* plan, int64_t n, int64_t 
   if (int rc = check_rows_plan(plan, n, vocab, width)) return rc;
   if (vocab == 0 || (n == 0 && accumulate)) return HPSPMM_OK;
   hipStream_t st = (hipStream_t)stream;
-  Sorted sorted{};
-  if (int rc = sort_rows(plan, n, vocab, d_ids, id_type, nullptr, nullptr, st, &sorted)) return rc;
   const int64_t grad_size = dtype_size(grad_type), table_size = dtype_size(table_type);
+  // Rows that no id points at become zeros either in the launches of the sort, which leave most of the chip idle but know
+  // of no row yet (so every row is filled), or beside the sums, where those that get one are left out.  The first hides
+  // the sort behind the fill, 20 to 40 us, and writes at most min(n, vocab) rows twice.
+  const bool early = !accumulate && std::min(n, vocab) * width * table_size <= (int64_t)192 << 20;
+  ZeroRows zero;
+  if (early) {
+    zero.at = (char*)d_table;
+    zero.rows = vocab;
+    zero.bytes = width * table_size;
+    zero.pitch = ld_table * table_size;
+    zero.flat = ld_table == width;
+  }
+  Sorted sorted{};
+  if (int rc = sort_rows(plan, n, vocab, d_ids, id_type, nullptr, nullptr, zero, st, &sorted)) return rc;
   const SumShape s = sum_shape(n, width, 16 / grad_size);
   if (2 * s.chunks * s.pitch > plan->carry_floats) return fail(HPSPMM_ERR_INVALID_ARG, "the plan's workspace is too small");
   const int64_t per_block = s.tpr_log2 < 6 ? hpspmm::kBlock >> s.tpr_log2 : 1;
   const int64_t sum_blocks = ceil_div(s.chunks, per_block);
-  const int64_t zero_blocks = accumulate ? 0 : std::min<int64_t>(ceil_div(vocab, hpspmm::kZeroRows), 1 << 20);
+  const int64_t zero_blocks = accumulate || early ? 0 : std::min<int64_t>(ceil_div(vocab, hpspmm::kZeroRows), 1 << 20);
   const unsigned threads = s.tpr_log2 < 6 ? hpspmm::kBlock : 1u << s.tpr_log2;
-  const bool aligned = aligned_to(d_grad, 16) && aligned_to(d_table, 16) && ld_grad * grad_size % 16 == 0 && ld_table * table_size % 16 == 0;
+  const bool whole = aligned_to(d_grad, 16) && aligned_to(d_table, 16) && ld_grad * grad_size % 16 == 0 &&
+                     ld_table * table_size % 16 == 0 && width * grad_size % 16 == 0;
   const hpspmm::SumArgs g{n, (uint32_t)vocab, (int32_t)width, (int32_t)s.pitch, sorted.keys, sorted.rows, d_grad, ld_grad, scale,
                           d_table, ld_table, accumulate != 0, plan->d_carry, s.chunk_log2, s.tpr_log2, s.chunks, (unsigned)sum_blocks,
                           (unsigned)zero_blocks};
-  const dim3 fix_grid((unsigned)ceil_div(s.chunks, hpspmm::kFixChunks), (unsigned)ceil_div(width, 256));
+  const dim3 fix_grid((unsigned)s.chunks, (unsigned)ceil_div(width, 256));
   dispatch_dtype(table_type, [&](auto o) {
     using TO = decltype(o);
     dispatch_dtype(grad_type, [&](auto t) {
@@ -292,16 +337,16 @@ HPSPMM_API int hpspmm_embedding_grad(hpspmm_rows_plan* plan, int64_t n, int64_t 
         hipLaunchKernelGGL(kernel, dim3((unsigned)(sum_blocks + zero_blocks), (unsigned)s.col_tiles), dim3(threads), 0, st, g);
       };
       if (s.tpr_log2 >= 6) {
-        if (aligned) launch(hpspmm::embedding_sum_kernel<T, TO, true, true>);
+        if (whole) launch(hpspmm::embedding_sum_kernel<T, TO, true, true>);
         else launch(hpspmm::embedding_sum_kernel<T, TO, false, true>);
       } else {
-        if (aligned) launch(hpspmm::embedding_sum_kernel<T, TO, true, false>);
+        if (whole) launch(hpspmm::embedding_sum_kernel<T, TO, true, false>);
         else launch(hpspmm::embedding_sum_kernel<T, TO, false, false>);
       }
       return HPSPMM_OK;
     });
     if (s.chunks > 1) {
-      if (aligned) hipLaunchKernelGGL((hpspmm::embedding_fix_kernel<TO, true>), fix_grid, dim3(hpspmm::kBlock), 0, st, g);
+      if (whole) hipLaunchKernelGGL((hpspmm::embedding_fix_kernel<TO, true>), fix_grid, dim3(hpspmm::kBlock), 0, st, g);
       else hipLaunchKernelGGL((hpspmm::embedding_fix_kernel<TO, false>), fix_grid, dim3(hpspmm::kBlock), 0, st, g);
     }
     return HPSPMM_OK;
