@@ -55,48 +55,36 @@ __global__ __launch_bounds__(kBlock) void embedding_lookup_kernel(int64_t n, uin
   }
 }
 
-// Rows of zeros, for the launches that have workgroups to spare: rows [0, rows) of `bytes` + `tail` bytes each, `pitch`
-// bytes apart, by `blocks` workgroups from workgroup `first` on.  An all-zero word is a zero of every element type.
+// Rows of zeros, for the launches that have workgroups to spare: rows [0, rows) of `bytes` bytes (the last one of
+// `last`), `pitch` bytes apart, by `blocks` workgroups from workgroup `first` on, 2^tpr_log2 threads a row.  An all-zero
+// word is a zero of every element type.
 struct ZeroFill {
   char* at;
-  int64_t rows, bytes, pitch;
+  int64_t rows, bytes, last, pitch;
   unsigned first, blocks;
-  int unit, tail;  // bytes of a store: 16, 4 or 2 (address, `bytes` and pitch are multiples of it); what is left, 0 ... 14
+  int unit_log2, tpr_log2;  // bytes of a store: 16, 4 or 2; address and pitch are multiples of it
 };
 template <class U>
 __device__ __forceinline__ void fill_units(const ZeroFill& z) {
-  const int64_t rows = z.rows;
-  const int64_t units = z.bytes / (int64_t)sizeof(U);
+  const int per_block = (int)blockDim.x >> z.tpr_log2, tpr = 1 << z.tpr_log2;
   const U zero{};
-  if (units >= (int64_t)blockDim.x * 4) {
-    // whole workgroups along a row, 4 stores a thread and step
-    const int64_t pieces = (units + 4 * (int64_t)blockDim.x - 1) / (4 * (int64_t)blockDim.x);
-    for (int64_t p = (int64_t)blockIdx.x - z.first; p < rows * pieces; p += z.blocks) {
-      const int64_t r = p / pieces, u0 = (p - r * pieces) * 4 * blockDim.x + threadIdx.x;
-      U* row = (U*)(z.at + r * z.pitch);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int64_t u = u0 + q * (int64_t)blockDim.x;
-        if (u < units) row[u] = zero;
-      }
-    }
-  } else {
-    const int64_t all = rows * units;  // (none where a row is shorter than a store)
-    for (int64_t i = ((int64_t)blockIdx.x - z.first) * blockDim.x + threadIdx.x; i < all; i += (int64_t)z.blocks * blockDim.x) {
-      const int64_t r = i / units;
-      ((U*)(z.at + r * z.pitch))[i - r * units] = zero;
-    }
+  for (int64_t r = (int64_t)(blockIdx.x - z.first) * per_block + ((int)threadIdx.x >> z.tpr_log2); r < z.rows;
+       r += (int64_t)z.blocks * per_block) {
+    char* row = z.at + r * z.pitch;
+    const int64_t bytes = r + 1 == z.rows ? z.last : z.bytes;
+    const int64_t units = bytes >> z.unit_log2;
+    const int t = (int)threadIdx.x & (tpr - 1);
+#pragma unroll 4
+    for (int64_t u = t; u < units; u += tpr) ((U*)row)[u] = zero;
+    if (t == 0)
+#pragma unroll 1
+      for (int64_t b = units << z.unit_log2; b < bytes; b += 2) *(uint16_t*)(row + b) = 0;
   }
 }
 __device__ __forceinline__ void zero_fill(const ZeroFill& z) {
-  if (z.unit == 16) fill_units<uint4>(z);
-  else if (z.unit == 4) fill_units<uint32_t>(z);
+  if (z.unit_log2 == 4) fill_units<uint4>(z);
+  else if (z.unit_log2 == 2) fill_units<uint32_t>(z);
   else fill_units<uint16_t>(z);
-  const int64_t left = z.rows * (z.tail / 2);
-  for (int64_t i = ((int64_t)blockIdx.x - z.first) * blockDim.x + threadIdx.x; i < left; i += (int64_t)z.blocks * blockDim.x) {
-    const int64_t r = i / (z.tail / 2);
-    ((uint16_t*)(z.at + r * z.pitch + z.bytes))[i - r * (z.tail / 2)] = 0;
-  }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -344,30 +332,19 @@ __global__ __launch_bounds__(kDigitThreads) void digit_scatter_kernel(int64_t n,
 
 constexpr int kSumFlight = 8;  // rows in flight
 
-// kWhole: rows at multiples of 16 bytes whose 16-byte pieces are all whole; otherwise any alignment and length.
-template <class T, bool kWhole>
-__device__ __forceinline__ void load_row(const T* p, int there, float (&v)[kPer16<T>]) {
-  if (kWhole || there >= kPer16<T>) {
-    load16<kWhole>(p, v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kPer16<T>; ++i) v[i] = i < there ? (float)p[i] : 0.f;
-  }
-}
-
 // Sorted keys and rows, as the kernel finds them: reads at addresses that a whole workgroup shares go through scalar
 // registers.
 template <class T>
 using Fixed = const __attribute__((address_space(4))) T*;
 
-// at[0 .. there) = (accumulate ? at : 0) + scale * v.
+// Elements [lo, hi) of at[0 .. kN) = (accumulate ? at : 0) + scale * v.  kWhole: all of them, at a multiple of their size.
 template <class TO, int kN, bool kWhole>
-__device__ __forceinline__ void store_sum(TO* at, int there, const float (&v)[kN], float scale, int accumulate) {
+__device__ __forceinline__ void store_sum(TO* at, int lo, int hi, const float (&v)[kN], float scale, int accumulate) {
   constexpr int kPart = kN < kPer16<TO> ? kN : kPer16<TO>;
+  if (kWhole || (lo == 0 && hi >= kN)) {
 #pragma unroll
-  for (int p = 0; p < kN; p += kPart) {
-    float out[kPart];
-    if (kWhole || there >= p + kPart) {
+    for (int p = 0; p < kN; p += kPart) {
+      float out[kPart];
 #pragma unroll
       for (int i = 0; i < kPart; ++i) out[i] = scale * v[p + i];
       if (accumulate) {
@@ -376,13 +353,21 @@ __device__ __forceinline__ void store_sum(TO* at, int there, const float (&v)[kN
         for (int i = 0; i < kPart; ++i) out[i] += (float)old[i];
       }
       store_n<kWhole, TO, kPart>(at + p, out);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kPart; ++i)
-        if (p + i < there) at[p + i] = (TO)((accumulate ? (float)at[p + i] : 0.f) + scale * v[p + i]);
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kN; ++i)
+      if (i >= lo && i < hi) {
+        float out = scale * v[i];
+        if (accumulate) out += (float)at[i];
+        at[i] = (TO)out;
+      }
   }
 }
+
+// How the rows lie: whole 16-byte pieces at multiples of 16 bytes; any alignment and length, but at least one piece (the
+// last thread of a row then reads the row's last 16 bytes and leaves out what its neighbour owns); shorter rows.
+enum RowForm { kRowWhole = 0, kRowLoose = 1, kRowShort = 2 };
 
 struct SumArgs {
   int64_t n;
@@ -405,9 +390,10 @@ struct SumArgs {
 
 constexpr int kZeroRows = 64;  // rows of the table a workgroup looks at for that
 
-template <class T, class TO, bool kWhole, bool kWide>
+template <class T, class TO, int kForm, bool kWide>
 __global__ __launch_bounds__(kBlock) void embedding_sum_kernel(SumArgs g) {
   constexpr int V = kPer16<T>;
+  constexpr bool kWhole = kForm == kRowWhole;
   const int tpr = 1 << g.tpr_log2;
   if (blockIdx.x >= g.sum_blocks) {
     // (all column tiles of a row by one workgroup)
@@ -427,61 +413,62 @@ __global__ __launch_bounds__(kBlock) void embedding_sum_kernel(SumArgs g) {
         rows &= rows - 1;
         TO* row = (TO*)g.d_table + (v0 + r) * g.ld_table;
         for (int c = (int)threadIdx.x * kPart; c < g.width; c += (int)blockDim.x * kPart)
-          store_sum<TO, kPart, false>(row + c, g.width - c, zero, 0.f, 0);
+          store_sum<TO, kPart, false>(row + c, 0, g.width - c, zero, 0.f, 0);
       }
     }
     return;
   }
   const int64_t c = kWide ? (int64_t)blockIdx.x : ((int64_t)blockIdx.x << (8 - g.tpr_log2)) + ((int)threadIdx.x >> g.tpr_log2);
-  const int col = ((int)blockIdx.y * tpr + ((int)threadIdx.x & (tpr - 1))) * V;
-  const int there = g.width - col;
-  if (c >= g.chunks || there <= 0) return;
+  const int own = ((int)blockIdx.y * tpr + ((int)threadIdx.x & (tpr - 1))) * V;  // first column of this thread's
+  if (c >= g.chunks || own >= g.width) return;
+  const int col = kForm == kRowLoose ? min(own, g.width - V) : own;              // first column that it reads
+  const int lo = own - col, hi = kForm == kRowShort ? g.width : V;
   const int64_t begin = c << g.chunk_log2, end = min(begin + ((int64_t)1 << g.chunk_log2), g.n);
   const Fixed<uint32_t> keys = (Fixed<uint32_t>)(uintptr_t)g.keys;
   const Fixed<int32_t> pos = (Fixed<int32_t>)(uintptr_t)g.pos;
   uint32_t cur = keys[begin];
-  if (cur >= g.vocab) return;
-  bool open = begin > 0 && keys[begin - 1] == cur;  // the sum began in an earlier chunk
+  bool open = keys[begin > 0 ? begin - 1 : 0] == cur && begin > 0;  // the sum began in an earlier chunk
   float acc[V] = {};
   const T* grad = (const T*)g.grad + col;
   auto close = [&](int slot) {
-    if (slot >= 0) {
-      float* at = g.carry + (2 * c + slot) * (int64_t)g.pitch + col;
-      store_sum<float, V, true>(at, g.pitch - col, acc, 1.f, 0);
-    } else {
-      store_sum<TO, V, kWhole>((TO*)g.d_table + (int64_t)cur * g.ld_table + col, there, acc, g.scale, g.accumulate);
-    }
+    if (slot >= 0) store_sum<float, V, kWhole>(g.carry + (2 * c + slot) * (int64_t)g.pitch + col, lo, hi, acc, 1.f, 0);
+    else store_sum<TO, V, kWhole>((TO*)g.d_table + (int64_t)cur * g.ld_table + col, lo, hi, acc, g.scale, g.accumulate);
   };
-  bool done = false;
-  for (int64_t q0 = begin; q0 < end && !done; q0 += kSumFlight) {
+  for (int64_t q0 = begin; q0 < end && cur < g.vocab; q0 += kSumFlight) {
+    // (all loads are asked for before the first is used: none is conditional, behind the end the last row is read again)
     uint32_t key[kSumFlight];
-    float row[kSumFlight][V];
+    int32_t from[kSumFlight];
+    typename Pack<T, V, true>::type row[kSumFlight];
 #pragma unroll
     for (int u = 0; u < kSumFlight; ++u) {
-      key[u] = q0 + u < end ? keys[q0 + u] : g.vocab;
-      if (key[u] < g.vocab) load_row<T, kWhole>(grad + (int64_t)pos[q0 + u] * g.ld_grad, there, row[u]);
+      const int64_t q = min(q0 + u, end - 1);
+      key[u] = keys[q];
+      from[u] = pos[q];
+    }
+    if constexpr (kWide) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < kSumFlight; ++u) {
+      const T* p = grad + (int64_t)from[u] * g.ld_grad;
+      if constexpr (kForm == kRowShort) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) row[u][i] = i < hi ? p[i] : (T)0.f;
+      } else {
+        row[u] = *reinterpret_cast<const typename Pack<T, V, kWhole>::type*>(p);
+      }
     }
 #pragma unroll
     for (int u = 0; u < kSumFlight; ++u) {
-      if (done) break;
+      if (q0 + u >= end) break;
       if (key[u] != cur) {
-        // (behind the chunk's last row, the vocabulary's end stands for what follows)
-        if (q0 + u >= end) {
-          done = true;
-          break;
-        }
         close(open ? 0 : -1);
         open = false;
         cur = key[u];
+        if (cur >= g.vocab) break;
 #pragma unroll
         for (int i = 0; i < V; ++i) acc[i] = 0.f;
-        if (cur >= g.vocab) {
-          done = true;
-          break;
-        }
       }
 #pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] += row[u][i];
+      for (int i = 0; i < V; ++i) acc[i] += (float)row[u][i];
     }
   }
   if (cur >= g.vocab) return;
@@ -531,7 +518,7 @@ __global__ __launch_bounds__(kBlock) void embedding_fix_kernel(SumArgs g) {
   for (int w = 1; w < kWavesPerBlock; ++w)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] += s_part[w][lane][i];
-  store_sum<TO, 4, kWhole>((TO*)g.d_table + (int64_t)key * g.ld_table + col, there, acc, g.scale, g.accumulate);
+  store_sum<TO, 4, kWhole>((TO*)g.d_table + (int64_t)key * g.ld_table + col, 0, there, acc, g.scale, g.accumulate);
 }
 
 }  // namespace hpspmm

@@ -71,26 +71,28 @@ struct Sorted {
 // The rows of a table that become zeros, cut into stretches for launches to come.
 struct ZeroRows {
   char* at = nullptr;
-  int64_t rows = 0, bytes = 0, pitch = 0;
-  bool flat = false;  // one stretch of memory, rows * bytes long
+  int64_t rows = 0, bytes = 0, last = 0, pitch = 0;
+  ZeroRows() = default;
+  ZeroRows(void* table, int64_t n, int64_t row_bytes, int64_t row_pitch)
+      : at((char*)table), rows(n), bytes(row_bytes), last(row_bytes), pitch(row_pitch) {
+    if (row_bytes == row_pitch && n > 0) {  // one stretch of memory, in pieces of 16 KB
+      const int64_t all = n * row_bytes;
+      bytes = pitch = 16384;
+      rows = ceil_div(all, bytes);
+      last = all - (rows - 1) * bytes;
+    }
+  }
   // The next of `left` stretches, for a launch of `first` workgroups of `threads` threads; *grid = the workgroups in all.
   hpspmm::ZeroFill next(int64_t first, int left, int threads, unsigned* grid) {
-    hpspmm::ZeroFill z{at, 0, bytes, pitch, (unsigned)first, 0, 16, 0};
     const int64_t share = ceil_div(rows, left);
-    if (flat) {
-      z.rows = share > 0;
-      z.bytes = share * bytes;
-      z.pitch = 0;
-    } else {
-      z.rows = share;
-    }
+    hpspmm::ZeroFill z{at, share, bytes, share == rows ? last : bytes, pitch, (unsigned)first, 0, 4, 0};
     at += share * pitch;
     rows -= share;
     const int64_t apart = (int64_t)(uintptr_t)z.at | z.pitch;
-    z.unit = apart % 16 == 0 ? 16 : apart % 4 == 0 ? 4 : 2;
-    z.tail = (int)(z.bytes % z.unit);
-    z.bytes -= z.tail;
-    z.blocks = (unsigned)std::min<int64_t>(ceil_div(z.rows * (z.bytes + z.tail), (int64_t)z.unit * threads * 4), 4096);
+    z.unit_log2 = apart % 16 == 0 ? 4 : apart % 4 == 0 ? 2 : 1;
+    // four stores a thread
+    while ((1 << z.tpr_log2) < threads && ((int64_t)4 << (z.tpr_log2 + z.unit_log2)) < bytes) ++z.tpr_log2;
+    z.blocks = (unsigned)std::min<int64_t>(ceil_div(share << z.tpr_log2, threads), 4096);
     *grid = (unsigned)first + z.blocks;
     return z;
   }
@@ -154,7 +156,7 @@ struct SumShape {
   int tpr_log2, chunk_log2;
   int64_t col_tiles, chunks, pitch;
 };
-constexpr int kMinChunkLog2 = 3, kMaxChunkLog2 = 7;
+constexpr int kMinChunkLog2 = 2, kMaxChunkLog2 = 7;
 SumShape sum_shape(int64_t n, int64_t width, int64_t per16) {
   SumShape s{};
   const int64_t vecs = ceil_div(width, per16);
@@ -307,14 +309,7 @@ HPSPMM_API int hpspmm_embedding_grad(hpspmm_rows_plan* plan, int64_t n, int64_t 
   // of no row yet (so every row is filled), or beside the sums, where those that get one are left out.  The first hides
   // the sort behind the fill, 20 to 40 us, and writes at most min(n, vocab) rows twice.
   const bool early = !accumulate && std::min(n, vocab) * width * table_size <= (int64_t)192 << 20;
-  ZeroRows zero;
-  if (early) {
-    zero.at = (char*)d_table;
-    zero.rows = vocab;
-    zero.bytes = width * table_size;
-    zero.pitch = ld_table * table_size;
-    zero.flat = ld_table == width;
-  }
+  const ZeroRows zero = early ? ZeroRows(d_table, vocab, width * table_size, ld_table * table_size) : ZeroRows();
   Sorted sorted{};
   if (int rc = sort_rows(plan, n, vocab, d_ids, id_type, nullptr, nullptr, zero, st, &sorted)) return rc;
   const SumShape s = sum_shape(n, width, 16 / grad_size);
@@ -336,13 +331,12 @@ HPSPMM_API int hpspmm_embedding_grad(hpspmm_rows_plan* plan, int64_t n, int64_t 
       auto launch = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)(sum_blocks + zero_blocks), (unsigned)s.col_tiles), dim3(threads), 0, st, g);
       };
-      if (s.tpr_log2 >= 6) {
-        if (whole) launch(hpspmm::embedding_sum_kernel<T, TO, true, true>);
-        else launch(hpspmm::embedding_sum_kernel<T, TO, false, true>);
-      } else {
-        if (whole) launch(hpspmm::embedding_sum_kernel<T, TO, true, false>);
-        else launch(hpspmm::embedding_sum_kernel<T, TO, false, false>);
-      }
+      using hpspmm::embedding_sum_kernel;
+      if (width < 16 / grad_size) launch(embedding_sum_kernel<T, TO, hpspmm::kRowShort, false>);
+      else if (s.tpr_log2 >= 6 && whole) launch(embedding_sum_kernel<T, TO, hpspmm::kRowWhole, true>);
+      else if (s.tpr_log2 >= 6) launch(embedding_sum_kernel<T, TO, hpspmm::kRowLoose, true>);
+      else if (whole) launch(embedding_sum_kernel<T, TO, hpspmm::kRowWhole, false>);
+      else launch(embedding_sum_kernel<T, TO, hpspmm::kRowLoose, false>);
       return HPSPMM_OK;
     });
     if (s.chunks > 1) {
