@@ -23,7 +23,14 @@ struct GroupedArgs {
   void* c;  // y, dx, dw
   int64_t ldc, stride_c;
   int accumulate;
+  int splits;    // gradient of w: parts that the rows of a group are cut into
+  float* parts;  // [splits * tiles][kSplitEdge * kSplitEdge] their sums
 };
+
+// Where the gradient of w has few tiles, the rows of each group are cut into parts: tiles of this edge, at most so many
+// of them times parts (32 MB of sums).
+constexpr int kSplitEdge = 128;
+constexpr int64_t kSplitTiles = 512;
 
 // Rows [begin, end) of a group; offsets that are no partition of the rows give other products, never an access
 // outside the operands.
@@ -91,6 +98,33 @@ __device__ __forceinline__ void panel_tile(int64_t t, int64_t row_tiles, int col
   const int64_t in = t - panel * row_tiles * kPanel;
   row = in / wide;
   col = (int)panel * kPanel + (int)(in - row * wide);
+}
+
+// dw = (accumulate ? dw : 0) + the parts' sums, added in their order.  A workgroup sums 1024 elements of one tile.
+template <class TO>
+__global__ __launch_bounds__(kBlock) void grouped_join_kernel(GroupedArgs g, int col_tiles) {
+  const int64_t t = blockIdx.x, tiles = gridDim.x;
+  const int row_tiles = (g.m + kSplitEdge - 1) / kSplitEdge;
+  const int64_t e = t / (row_tiles * col_tiles);
+  int64_t mt;
+  int nt;
+  panel_tile(t - e * row_tiles * col_tiles, row_tiles, col_tiles, mt, nt);
+  const int at = ((int)blockIdx.y * kBlock + (int)threadIdx.x) * 4;
+  const int64_t row = mt * kSplitEdge + at / kSplitEdge;
+  const int col = nt * kSplitEdge + at % kSplitEdge;
+  if (row >= g.m || col >= g.k) return;
+  float v[4] = {};
+#pragma unroll 4
+  for (int s = 0; s < g.splits; ++s) {
+    float part[4];
+    load16<true>(g.parts + (s * tiles + t) * (kSplitEdge * kSplitEdge) + at, part);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += part[i];
+  }
+  TO* out = (TO*)g.c + e * g.stride_c + row * g.ldc + col;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (col + i < g.k) out[i] = (TO)(v[i] + (g.accumulate ? (float)out[i] : 0.f));
 }
 
 }  // namespace hpspmm

@@ -41,6 +41,33 @@ bool chunked(const void* p, int64_t ld, int64_t stride, int64_t width, int64_t s
   return aligned_to(p, 16) && ld * size % 16 == 0 && stride * size % 16 == 0 && width * size % 16 == 0 && ld < ((int64_t)1 << 21);
 }
 
+// Output tiles of edge `edge` that a product can be expected to have: every group ends half way through a tile.
+int64_t expected_tiles(int mode, const hpspmm::GroupedArgs& g, int64_t edge) {
+  const int64_t cols = ceil_div(mode == hpspmm::kForward ? g.m : g.k, edge);
+  if (mode == hpspmm::kGradW) return cols * g.groups * ceil_div(g.m, edge);
+  return cols * std::max<int64_t>(1, std::min(g.rows, g.rows / edge + g.groups / 2));
+}
+
+// Edge of the output tiles, 256 (16-bit operands at multiples of 16 bytes), 128 or 64: rate of the tile times the share
+// of the chip that the last round of tiles leaves busy.  Rates of 16-bit products of 32768 x 2048 x 4096 over 32 groups:
+// 950, 800 and 500 TFLOP/s; a CU holds 1, 2 and 2 of the workgroups.  bf16, rows x groups x k x m, 64 / 128 / 256 in us:
+// 2000 x 8 x 1024 x 1024 16 / 16 / 32, 8192 x 8 x 1024 x 1024 41 / 34 / 34, 8192 x 8 x 2048 x 2048 119 / 89 / 109.
+int tile_edge(int mode, const hpspmm::GroupedArgs& g, bool large) {
+  const struct { int edge; int64_t slots; double rate; } kinds[] = {{256, 256, 9.5}, {128, 512, 8.0}, {64, 512, 5.0}};
+  int best = 64;
+  double most = 0;
+  for (const auto& q : kinds) {
+    if (q.edge == 256 && !large) continue;
+    const int64_t tiles = expected_tiles(mode, g, q.edge);
+    const double score = q.rate * (double)tiles / (double)(ceil_div(tiles, q.slots) * q.slots);
+    if (score > most) {
+      most = score;
+      best = q.edge;
+    }
+  }
+  return best;
+}
+
 template <class T, class TO, int kMode, int kBM, int kBN, int kWM, int kWN, bool kDirect, int kC, int kStages>
 int launch_tiles(const hpspmm::GroupedArgs& g, hipStream_t st) {
   const int64_t n_out = kMode == hpspmm::kForward ? g.m : g.k;
@@ -54,8 +81,35 @@ int launch_tiles(const hpspmm::GroupedArgs& g, hipStream_t st) {
   return HPSPMM_OK;
 }
 
+// Parts that the rows of every group are cut into for the gradient of the weights, 1 = none: where there are few output
+// tiles and long groups, as many as give every slot of the chip a tile, each of at least 4 steps of the mean group.
+int row_splits(const hpspmm::GroupedArgs& g, int64_t depth) {
+  const int64_t tiles = expected_tiles(hpspmm::kGradW, g, hpspmm::kSplitEdge);
+  const int64_t steps = g.rows / g.groups / depth;
+  return (int)std::max<int64_t>(1, std::min(hpspmm::kSplitTiles / std::max<int64_t>(tiles, 1), steps / 4));
+}
+
+// The gradient of the weights in parts: sums in 32 bits of every part and tile to the plan's workspace, then their sum.
+template <class T, class TO>
+int launch_split(hpspmm::GroupedArgs g, int splits, bool direct, hipStream_t st) {
+  g.splits = splits;
+  constexpr int E = hpspmm::kSplitEdge;
+  const int64_t col_tiles = ceil_div(g.k, E), tiles = g.groups * ceil_div(g.m, E) * col_tiles;
+  const unsigned grid = (unsigned)(ceil_div(tiles * splits, hpspmm::kXcds) * hpspmm::kXcds);
+  if (direct)
+    hipLaunchKernelGGL((hpspmm::grouped_tile_kernel<T, TO, hpspmm::kGradW, E, E, 2, 2, true, 8, 2, true>), dim3(grid), dim3(256), 0,
+                       st, g, (int)col_tiles);
+  else
+    hipLaunchKernelGGL((hpspmm::grouped_tile_kernel<T, TO, hpspmm::kGradW, E, E, 2, 2, false, 8, 2, true>), dim3(grid), dim3(256), 0,
+                       st, g, (int)col_tiles);
+  hipLaunchKernelGGL((hpspmm::grouped_join_kernel<TO>), dim3((unsigned)tiles, E * E / (4 * hpspmm::kBlock)), dim3(hpspmm::kBlock), 0, st,
+                     g, (int)col_tiles);
+  return HPSPMM_OK;
+}
+
 template <int kMode>
 int launch_grouped(const hpspmm::GroupedArgs& g, int dtype, int out_type, hipStream_t st) {
+  if (g.groups == 0 || (kMode != hpspmm::kGradW && g.rows == 0)) return HPSPMM_OK;
   const int64_t size = dtype_size(dtype);
   const int64_t wide_a = kMode == hpspmm::kForward ? g.k : g.m;
   const bool direct = chunked(g.a, g.lda, 0, wide_a, size) && chunked(g.b, g.ldb, g.stride_b, g.k, size);
@@ -64,11 +118,19 @@ int launch_grouped(const hpspmm::GroupedArgs& g, int dtype, int out_type, hipStr
     return dispatch_dtype(out_type, [&](auto o) {
       using TO = decltype(o);
       if constexpr (std::is_same_v<T, TO> || (kMode == hpspmm::kGradW && std::is_same_v<TO, float>)) {
-        if (!direct) return launch_tiles<T, TO, kMode, 128, 128, 2, 2, false, 8, 2>(g, st);
-        if constexpr (sizeof(T) == 2) {
-          if (g.rows >= 4096) return launch_tiles<T, TO, kMode, 256, 256, 2, 4, true, 8, 2>(g, st);
+        if constexpr (kMode == hpspmm::kGradW) {
+          const int splits = row_splits(g, 128 / (int64_t)sizeof(T));
+          if (splits > 1) return launch_split<T, TO>(g, splits, direct, st);
         }
-        return launch_tiles<T, TO, kMode, 128, 128, 2, 2, true, 8, 2>(g, st);
+        const int edge = tile_edge(kMode, g, sizeof(T) == 2 && direct);
+        if constexpr (sizeof(T) == 2) {
+          if (edge == 256) return launch_tiles<T, TO, kMode, 256, 256, 2, 4, true, 8, 2>(g, st);
+        }
+        if (edge == 128)
+          return direct ? launch_tiles<T, TO, kMode, 128, 128, 2, 2, true, 8, 2>(g, st)
+                        : launch_tiles<T, TO, kMode, 128, 128, 2, 2, false, 8, 2>(g, st);
+        return direct ? launch_tiles<T, TO, kMode, 64, 64, 2, 2, true, 8, 4>(g, st)
+                      : launch_tiles<T, TO, kMode, 64, 64, 2, 2, false, 8, 2>(g, st);
       } else {
         return fail(HPSPMM_ERR_INVALID_ARG, "no product of these types");
       }
@@ -88,7 +150,7 @@ HPSPMM_API int hpspmm_grouped_mm(int64_t rows, int64_t groups, int64_t k, int64_
   if (int rc = check_matrix("d_x", d_x, rows, k, ld_x, dtype)) return rc;
   if (int rc = check_weights("d_w", d_w, groups, k, m, ld_w, stride_w, dtype, false)) return rc;
   if (int rc = check_matrix("d_y", d_y, rows, m, ld_y, dtype)) return rc;
-  const hpspmm::GroupedArgs g{rows, groups, (int32_t)k, (int32_t)m, d_offsets, d_x, ld_x, d_w, ld_w, stride_w, d_y, ld_y, 0, 0};
+  const hpspmm::GroupedArgs g{rows, groups, (int32_t)k, (int32_t)m, d_offsets, d_x, ld_x, d_w, ld_w, stride_w, d_y, ld_y, 0, 0, 1, nullptr};
   return launch_grouped<hpspmm::kForward>(g, dtype, dtype, (hipStream_t)stream);
 }
 
@@ -99,7 +161,7 @@ HPSPMM_API int hpspmm_grouped_mm_grad_x(int64_t rows, int64_t groups, int64_t k,
   if (int rc = check_matrix("d_dy", d_dy, rows, m, ld_dy, dtype)) return rc;
   if (int rc = check_weights("d_w", d_w, groups, k, m, ld_w, stride_w, dtype, false)) return rc;
   if (int rc = check_matrix("d_dx", d_dx, rows, k, ld_dx, dtype)) return rc;
-  const hpspmm::GroupedArgs g{rows, groups, (int32_t)k, (int32_t)m, d_offsets, d_dy, ld_dy, d_w, ld_w, stride_w, d_dx, ld_dx, 0, 0};
+  const hpspmm::GroupedArgs g{rows, groups, (int32_t)k, (int32_t)m, d_offsets, d_dy, ld_dy, d_w, ld_w, stride_w, d_dx, ld_dx, 0, 0, 1, nullptr};
   return launch_grouped<hpspmm::kGradX>(g, dtype, dtype, (hipStream_t)stream);
 }
 
@@ -114,6 +176,7 @@ HPSPMM_API int hpspmm_grouped_mm_grad_w(hpspmm_rows_plan* plan, int64_t rows, in
   if (int rc = check_matrix("d_x", d_x, rows, k, ld_x, dtype)) return rc;
   if (int rc = check_weights("d_dw", d_dw, groups, k, m, ld_dw, stride_dw, dw_type, true)) return rc;
   if (int rc = check_rows_plan(plan, 0, 0, 0)) return rc;
-  const hpspmm::GroupedArgs g{rows, groups, (int32_t)k, (int32_t)m, d_offsets, d_dy, ld_dy, d_x, ld_x, 0, d_dw, ld_dw, stride_dw, accumulate != 0};
+  const hpspmm::GroupedArgs g{rows, groups, (int32_t)k, (int32_t)m, d_offsets, d_dy, ld_dy, d_x, ld_x, 0, d_dw, ld_dw, stride_dw, accumulate != 0,
+                              1, plan->d_split};
   return launch_grouped<hpspmm::kGradW>(g, dtype, dw_type, (hipStream_t)stream);
 }

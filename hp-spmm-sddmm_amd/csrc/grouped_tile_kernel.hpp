@@ -70,8 +70,8 @@ struct Operand {
 
   static __device__ __forceinline__ int swizzle(int r) {
     if constexpr (!kCol) return kC == 8 ? r & 7 : (r >> 2) & 3;
-    else if constexpr (kSize == 2) return ((r & 3) | ((r >> 1) & 4)) << 1;
-    else return ((r >> 2) & 3) << 2;
+    else if constexpr (kSize == 2) return (((r & 3) | ((r >> 1) & 4)) << 1) & (kRowChunks - 1);
+    else return (((r >> 2) & 3) << 2) & (kRowChunks - 1);
   }
   // Row of LDS and chunk of that row in memory that this thread's i-th chunk is.
   static __device__ __forceinline__ void place(int i, int& r, int& c) {
@@ -197,7 +197,7 @@ __device__ __forceinline__ int64_t xcd_tile(int64_t tiles) {
   return b / kXcds < per && t < tiles ? t : -1;
 }
 
-template <class T, class TO, int kMode, int kBM, int kBN, int kWM, int kWN, bool kDirect, int kC, int kStages>
+template <class T, class TO, int kMode, int kBM, int kBN, int kWM, int kWN, bool kDirect, int kC, int kStages, bool kSplit = false>
 __global__ __launch_bounds__(64 * kWM * kWN, 2) void grouped_tile_kernel(GroupedArgs g, int col_tiles) {
   constexpr int kThreads = 64 * kWM * kWN;
   using OpA = Operand<T, kMode == kGradW, kBM, kThreads, kDirect, kC>;
@@ -213,15 +213,25 @@ __global__ __launch_bounds__(64 * kWM * kWN, 2) void grouped_tile_kernel(Grouped
   OpA a;
   OpB b;
   TO* c;
+  float* out_part = nullptr;
   if constexpr (kMode == kGradW) {
     const int row_tiles = (g.m + kBM - 1) / kBM;
-    const int64_t t = xcd_tile(g.groups * row_tiles * col_tiles);
-    if (t < 0) return;
+    const int64_t tiles = g.groups * row_tiles * col_tiles;
+    const int64_t tp = xcd_tile(kSplit ? tiles * g.splits : tiles);
+    if (tp < 0) return;
+    const int64_t part = kSplit ? tp / tiles : 0, t = kSplit ? tp - part * tiles : tp;
     e = t / (row_tiles * col_tiles);
     int64_t mt;
     int nt;
     panel_tile(t - e * row_tiles * col_tiles, row_tiles, col_tiles, mt, nt);
     group_rows_of(g, e, row0, end);
+    if constexpr (kSplit) {
+      // the part's steps of the contraction
+      const int64_t per = ((end - row0 + kDepth - 1) / kDepth + g.splits - 1) / g.splits * kDepth;
+      row0 = min(row0 + part * per, end);
+      end = min(row0 + per, end);
+      out_part = g.parts + tp * (kBM * kBN);
+    }
     depth = end - row0;
     m_left = g.m - mt * kBM;
     n_left = n_out - (int64_t)nt * kBN;
@@ -342,6 +352,14 @@ __global__ __launch_bounds__(64 * kWM * kWN, 2) void grouped_tile_kernel(Grouped
   if constexpr (kDirect) wait_loads<0>();
 
   const int lane = threadIdx.x & 63;
+  if constexpr (kSplit) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+        *reinterpret_cast<float4_t*>(out_part + (am + i * 16 + (lane & 15)) * kBN + bn + j * 16 + (lane >> 4) * 4) = acc[i][j];
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
     const int row = am + i * 16 + (lane & 15);

@@ -2,6 +2,7 @@
 // holds their workspace.
 #include "row_ops.hpp"
 
+#include "grouped_kernels.hpp"
 #include "row_kernels.hpp"
 
 using namespace hpspmm_host;
@@ -201,7 +202,8 @@ HPSPMM_API int hpspmm_rows_plan_create(int64_t max_rows, int64_t max_ids, int64_
   // (fewer ids may make a digit of more bits)
   const int64_t hist = tiles << std::min<int>(hpspmm::kDigitBits, key_bits(max_ids)), scan = scan_scratch_words(hist);
   const int64_t carry = most_carry_floats(max_rows, max_width);
-  const int64_t words[] = {n, n, n, n, hist, scan, carry};
+  const int64_t split = hpspmm::kSplitTiles * hpspmm::kSplitEdge * hpspmm::kSplitEdge;
+  const int64_t words[] = {n, n, n, n, hist, scan, carry, split};
   int64_t bytes = 0;
   for (int64_t w : words) bytes += (w * 4 + 255) & ~(int64_t)255;
   if (hipMalloc((void**)&p->arena, (size_t)bytes) != hipSuccess) {
@@ -224,6 +226,7 @@ HPSPMM_API int hpspmm_rows_plan_create(int64_t max_rows, int64_t max_ids, int64_
   p->d_scan = (uint32_t*)take(scan);
   p->d_carry = (float*)take(carry);
   p->carry_floats = carry;
+  p->d_split = (float*)take(split);
   *plan_out = p;
   return HPSPMM_OK;
 }

@@ -16,6 +16,7 @@ struct hpspmm_rows_plan {
   uint32_t* d_scan = nullptr;
   float* d_carry = nullptr;                  // sums that cross chunks of the sorted rows
   int64_t carry_floats = 0;
+  float* d_split = nullptr;                  // sums of the parts of a gradient of the weights
 };
 
 namespace hpspmm_host {
