@@ -399,15 +399,29 @@ def csr_spmm_timed_launches(plan, rowptr, col, val, B, C, warmup=5, iters=50, st
 
 # ---- row operators -------------------------------------------------------------------------------------------------
 
-_dtypes = None  # {torch type: hpspmm_dtype}, {torch type: hpspmm_id_type}
+class _Torch:
+    """What the row operators need of torch, looked up once: their calls take microseconds."""
 
-
-def _types():
-    global _dtypes
-    if _dtypes is None:
+    def __init__(self):
         import torch
-        _dtypes = ({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}, {torch.int32: I32, torch.int64: I64})
-    return _dtypes
+        self.dtypes = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+        self.id_types = {torch.int32: I32, torch.int64: I64}
+        self.int32 = torch.int32
+        self.device = torch.cuda.device
+        self.current_device = torch.cuda.current_device
+        # the address of the current stream, without a Stream object around it (2.6 us) where torch has that
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        self.current_stream = raw or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+_torch = None
+
+
+def _with_torch():
+    global _torch
+    if _torch is None:
+        _torch = _Torch()
+    return _torch
 
 
 def _row_arg(t, name, device=None):
@@ -422,7 +436,7 @@ def _row_arg(t, name, device=None):
 def _rows_matrix(t, name, shape, device, dtype=None):
     """(address, leading dimension, hpspmm_dtype) of a matrix whose rows are contiguous."""
     _row_arg(t, name, device)
-    kind = _types()[0].get(t.dtype)
+    kind = _with_torch().dtypes.get(t.dtype)
     if kind is None or (dtype is not None and t.dtype != dtype):
         raise TypeError(f"{name} must be {dtype if dtype is not None else 'float32, bfloat16 or float16'}, got {t.dtype}")
     if tuple(t.shape) != shape:
@@ -436,16 +450,15 @@ def _rows_matrix(t, name, shape, device, dtype=None):
 
 def _row_ids(t, name, device=None):
     d = _row_arg(t, name, device)
-    kind = _types()[1].get(t.dtype)
+    kind = _with_torch().id_types.get(t.dtype)
     if kind is None or t.dim() != 1 or not t.is_contiguous():
         raise TypeError(f"{name} must be a contiguous vector of int32 or int64")
     return d, t.data_ptr(), kind
 
 
 def _offsets(t, name, entries, device):
-    import torch
     _row_arg(t, name, device)
-    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+    if t.dtype != _with_torch().int32 or t.dim() != 1 or not t.is_contiguous():
         raise TypeError(f"{name} must be a contiguous vector of int32")
     if t.numel() != entries:
         raise ValueError(f"{name} must have {entries} entries, got {t.numel()}")
@@ -454,13 +467,11 @@ def _offsets(t, name, entries, device):
 
 def _call_on(device, stream, function, *args):
     """function(*args, stream) with `device` current, on `stream` or that device's current one."""
-    import torch
-    if torch.cuda.current_device() == device.index:
-        st = torch.cuda.current_stream() if stream is None else stream
-        return check(function(*args, st.cuda_stream))
-    with torch.cuda.device(device):
-        st = torch.cuda.current_stream() if stream is None else stream
-        return check(function(*args, st.cuda_stream))
+    t, index = _with_torch(), device.index
+    if t.current_device() == index:
+        return check(function(*args, t.current_stream(index) if stream is None else stream.cuda_stream))
+    with t.device(index):
+        return check(function(*args, t.current_stream(index) if stream is None else stream.cuda_stream))
 
 
 class RowsPlan:
