@@ -9,7 +9,7 @@ namespace hpspmm {
 // out[i, :] = scale * table[ids[i], :], rows of zeros for ids outside the table.  A thread owns 16 bytes of a row;
 // 2^tpr_log2 adjacent threads share a row's column tile, a workgroup covers kRows rows one after the other, all of
 // whose loads are in flight together.
-template <class T, class Id, bool kAligned, int kRows>
+template <class T, class Id, bool kAligned, int kRows, bool kStream>
 __global__ __launch_bounds__(kBlock) void embedding_lookup_kernel(int64_t n, uint32_t vocab, int32_t width, int tpr_log2,
                                                                  const Id* __restrict__ ids, const T* __restrict__ table,
                                                                  int64_t ld_table, float scale, T* __restrict__ out,
@@ -42,7 +42,9 @@ __global__ __launch_bounds__(kBlock) void embedding_lookup_kernel(int64_t n, uin
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       const int64_t row = row0 + (int64_t)r * per_pass;
-      if (row < n) store_n<kAligned, T, V>(out + row * ld_out + col, v[r]);
+      if (row >= n) continue;
+      if constexpr (kStream) stream_n<kAligned, T, V>(out + row * ld_out + col, v[r]);
+      else store_n<kAligned, T, V>(out + row * ld_out + col, v[r]);
     }
   } else {
     for (int r = 0; r < kRows; ++r) {

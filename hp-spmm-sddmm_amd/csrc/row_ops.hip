@@ -256,6 +256,7 @@ HPSPMM_API int hpspmm_embedding_lookup(int64_t n, int64_t vocab, int64_t width, 
   const int64_t col_tiles = ceil_div(vecs, (int64_t)1 << tpr_log2);
   const int64_t per_pass = hpspmm::kBlock >> tpr_log2;
   const bool many = n * col_tiles >= 4 * per_pass * 1024;
+  const bool past_caches = aligned && many && n * width * size >= hpspmm::kStreamBytes && aligned_to(d_out, 128) && ld_out * size % 128 == 0;
   // (a launch holds fewer than 2^32 threads: 2^23 workgroups at a time)
   const int64_t per_block = per_pass * (many ? 4 : 1), per_launch = per_block << 23;
   dispatch_dtype(dtype, [&](auto t) {
@@ -270,13 +271,12 @@ HPSPMM_API int hpspmm_embedding_lookup(int64_t n, int64_t vocab, int64_t width, 
                              scale, (T*)d_out + r * ld_out, ld_out);
         }
       };
-      if (aligned) {
-        if (many) launch(hpspmm::embedding_lookup_kernel<T, Id, true, 4>);
-        else launch(hpspmm::embedding_lookup_kernel<T, Id, true, 1>);
-      } else {
-        if (many) launch(hpspmm::embedding_lookup_kernel<T, Id, false, 4>);
-        else launch(hpspmm::embedding_lookup_kernel<T, Id, false, 1>);
-      }
+      using hpspmm::embedding_lookup_kernel;
+      if (past_caches) launch(embedding_lookup_kernel<T, Id, true, 4, true>);
+      else if (aligned && many) launch(embedding_lookup_kernel<T, Id, true, 4, false>);
+      else if (aligned) launch(embedding_lookup_kernel<T, Id, true, 1, false>);
+      else if (many) launch(embedding_lookup_kernel<T, Id, false, 4, false>);
+      else launch(embedding_lookup_kernel<T, Id, false, 1, false>);
       return HPSPMM_OK;
     });
   });

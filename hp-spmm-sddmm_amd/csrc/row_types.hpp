@@ -40,6 +40,16 @@ __device__ __forceinline__ void store_n(T* p, const float* in) {
   *reinterpret_cast<typename Pack<T, kN, kAligned>::type*>(p) = v;
 }
 
+// The same past the caches: for outputs that do not fit them, in whole lines (pieces of lines cost more than they save).
+template <bool kAligned, class T, int kN>
+__device__ __forceinline__ void stream_n(T* p, const float* in) {
+  typename Pack<T, kN, true>::type v;
+#pragma unroll
+  for (int i = 0; i < kN; ++i) v[i] = (T)in[i];
+  __builtin_nontemporal_store(v, reinterpret_cast<typename Pack<T, kN, kAligned>::type*>(p));
+}
+constexpr int64_t kStreamBytes = (int64_t)64 << 20;  // outputs from this size on are written past the caches
+
 // Key of one id: the id itself, or `ids` for one outside [0, ids).
 template <class Id>
 __device__ __forceinline__ uint32_t id_key(Id id, uint32_t ids) {
