@@ -189,6 +189,9 @@ __device__ __forceinline__ void meet() {
   asm volatile("" ::: "memory");
 }
 
+// The largest part of `all` rows, halved as often as needed, that fits `room` rows.
+constexpr int whole_rows(int room, int all) { return all <= room ? all : whole_rows(room, all / 2); }
+
 // Workgroup -> output tile: the tiles in use are cut into one contiguous stretch for each XCD, so that the tiles that an
 // XCD works on at a time share rows of x and columns of w in its L2.
 __device__ __forceinline__ int64_t xcd_tile(int64_t tiles) {
@@ -197,15 +200,15 @@ __device__ __forceinline__ int64_t xcd_tile(int64_t tiles) {
   return b / kXcds < per && t < tiles ? t : -1;
 }
 
-template <class T, class TO, int kMode, int kBM, int kBN, int kWM, int kWN, bool kDirect, int kC, int kStages, bool kSplit = false>
+template <class T, class TO, int kMode, int kBM, int kBN, int kWM, int kWN, bool kDirect, int kC, int kStagesA, int kStagesB, bool kSplit = false>
 __global__ __launch_bounds__(64 * kWM * kWN, 2) void grouped_tile_kernel(GroupedArgs g, int col_tiles) {
   constexpr int kThreads = 64 * kWM * kWN;
   using OpA = Operand<T, kMode == kGradW, kBM, kThreads, kDirect, kC>;
   using OpB = Operand<T, kMode != kForward, kBN, kThreads, kDirect, kC>;
   using Frag = typename Mfma<T>::frag;
   constexpr int FM = kBM / kWM / 16, FN = kBN / kWN / 16, kDepth = OpA::kDepth;
-  constexpr int kStage = OpA::kBytes + OpB::kBytes;
-  __shared__ __attribute__((aligned(1024))) char lds[kStages * kStage];
+  constexpr int kLdsA = kStagesA * OpA::kBytes, kLds = kLdsA + kStagesB * OpB::kBytes;
+  __shared__ __attribute__((aligned(1024))) char lds[kLds];
 
   // the tile of the output, its operands, the length of the contraction
   int64_t e, row0 = 0, end = 0, depth, m_left, n_left;
@@ -262,12 +265,12 @@ __global__ __launch_bounds__(64 * kWM * kWN, 2) void grouped_tile_kernel(Grouped
   // The products of one step, sum by sum of 16 rows; `between(i)` after the i-th.  The next half of the step is read
   // while this one is multiplied.
   constexpr int H = kC / 4;
-  auto multiply = [&](const char* lds, auto between) {
+  auto multiply = [&](const char* lds_a, const char* lds_b, auto between) {
     Frag fa[H][FM], fb[H][FN];
 #pragma unroll
-    for (int j = 0; j < FN; ++j) fb[0][j] = OpB::fragment(lds + OpA::kBytes, bn + j * 16, 0);
+    for (int j = 0; j < FN; ++j) fb[0][j] = OpB::fragment(lds_b, bn + j * 16, 0);
 #pragma unroll
-    for (int i = 0; i < FM; ++i) fa[0][i] = OpA::fragment(lds, am + i * 16, 0);
+    for (int i = 0; i < FM; ++i) fa[0][i] = OpA::fragment(lds_a, am + i * 16, 0);
 #pragma unroll
     for (int h = 0; h < H; ++h)
 #pragma unroll
@@ -277,76 +280,83 @@ __global__ __launch_bounds__(64 * kWM * kWN, 2) void grouped_tile_kernel(Grouped
         for (int j = 0; j < FN; ++j) acc[i][j] = Mfma<T>::mul(fb[h][j], fa[h][i], acc[i][j]);
         between(h * FM + i);
         if (h + 1 < H) {
-          fa[h + 1][i] = OpA::fragment(lds, am + i * 16, h + 1);
-          if (i < FN) fb[h + 1][i] = OpB::fragment(lds + OpA::kBytes, bn + i * 16, h + 1);
+          fa[h + 1][i] = OpA::fragment(lds_a, am + i * 16, h + 1);
+          if (i < FN) fb[h + 1][i] = OpB::fragment(lds_b, bn + i * 16, h + 1);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
   };
 
-  // kStages steps in LDS: one is multiplied while the next ones are on their way.  The barrier at the head of a step says
-  // that its operands are there, and that nobody reads the stage before it any more, which the step brought in then
-  // takes.  Loads past the registers are counted: those of the kStages - 2 steps behind may still be under way (steps
-  // beyond the last one are asked for as well, as zeros, so that the count holds to the end).
-  static_assert(kDirect || kStages == 2, "loads through registers are one step ahead");
+  // Some steps of each operand in LDS: one is multiplied while the next ones are on their way.  The barrier at the head
+  // of a step says that its operands are there, and that nobody reads the step before it any more, whose places the steps
+  // brought in then take.  Loads past the registers are counted: those of later steps may still be under way (steps beyond
+  // the last one are asked for as well, as zeros, so that the count holds to the end).  One operand may be a step further
+  // ahead than the other: three steps of a and two of b fill the 160 KB of LDS in tiles of 256, and what is behind the
+  // next step keeps the loads flowing while that one is waited for.
+  static_assert(kStagesA == kStagesB || kStagesA == kStagesB + 1, "a is asked for after b, and at most a step further ahead");
+  static_assert(kDirect || (kStagesA == 2 && kStagesB == 2), "loads through registers are one step ahead");
   const int64_t steps = (depth + kDepth - 1) / kDepth;
   typename OpA::Chunk ra[kDirect ? 1 : OpA::kPer];
   typename OpB::Chunk rb[kDirect ? 1 : OpB::kPer];
   const uint32_t lds_wave = (uint32_t)(uintptr_t)(lds_char*)lds + (uint32_t)wave * 1024u;  // where this wavefront's chunks go
-  constexpr int kLoads = OpA::kPer + OpB::kPer;
   static_assert(FN <= FM, "the fragments of a half are read between the sums of the half before");
-  auto bring_direct = [&](int stage, int i) {
-    const uint32_t to = lds_wave + (uint32_t)(stage * kStage);
-    if (i < OpA::kPer) a.load_direct(to, i);
-    else b.load_direct(to + OpA::kBytes, i - OpA::kPer);
+  int next_a = 0, next_b = 0;  // steps asked for
+  auto ask_a = [&](int i) {
+    if (i == 0) a.end_after(depth - (int64_t)next_a * kDepth);
+    a.load_direct(lds_wave + (uint32_t)(next_a % kStagesA * OpA::kBytes), i);
+    if (i + 1 == OpA::kPer) {
+      a.base += a.step;
+      ++next_a;
+    }
+  };
+  auto ask_b = [&](int i) {
+    if (i == 0) b.end_after(depth - (int64_t)next_b * kDepth);
+    b.load_direct(lds_wave + (uint32_t)(kLdsA + next_b % kStagesB * OpB::kBytes), i);
+    if (i + 1 == OpB::kPer) {
+      b.base += b.step;
+      ++next_b;
+    }
+  };
+  auto ask_both = [&](bool with_b) {
+#pragma unroll
+    for (int i = 0; i < OpB::kPer; ++i)
+      if (with_b) ask_b(i);
+#pragma unroll
+    for (int i = 0; i < OpA::kPer; ++i) ask_a(i);
   };
   if (steps > 0) {
     if constexpr (kDirect) {
-      for (int s = 0; s < kStages - 1; ++s) {
-        a.end_after(depth - s * kDepth);
-        b.end_after(depth - s * kDepth);
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) bring_direct(s, i);
-        a.base += a.step;
-        b.base += b.step;
-      }
+      for (int s = 0; s < kStagesA - 1; ++s) ask_both(s >= kStagesA - kStagesB);
     } else {
       a.load_loose(ra, depth);
       b.load_loose(rb, depth);
       OpA::put(lds, ra);
-      OpB::put(lds + OpA::kBytes, rb);
+      OpB::put(lds + kLdsA, rb);
     }
   }
-  int stage = 0;
+  int at_a = 0, at_b = 0;  // places of the step at hand
   for (int64_t s = 0; s < steps; ++s) {
-    const int before = stage == 0 ? kStages - 1 : stage - 1;
     if constexpr (kDirect) {
-      wait_loads<(kStages - 2) * kLoads>();
+      wait_loads<(kStagesA - 2) * OpA::kPer + (kStagesB - 2) * OpB::kPer>();
       meet();
-      a.end_after(depth - (s + kStages - 1) * kDepth);
-      b.end_after(depth - (s + kStages - 1) * kDepth);
-      // the loads spread over the products: asked for in one go they would keep the wavefront waiting for its turn
-      multiply(lds + stage * kStage, [&](int i) {
-        constexpr int kSpread = 8;
-#pragma unroll
-        for (int q = 0; q < kSpread; ++q)
-          if (i * kSpread + q < kLoads) bring_direct(before, i * kSpread + q);
+      multiply(lds + at_a * OpA::kBytes, lds + kLdsA + at_b * OpB::kBytes, [&](int i) {
+        if (i == 0) ask_both(true);
       });
-      a.base += a.step;
-      b.base += b.step;
     } else {
       __syncthreads();
       if (s + 1 < steps) {
         a.load_loose(ra, depth - (s + 1) * kDepth);
         b.load_loose(rb, depth - (s + 1) * kDepth);
       }
-      multiply(lds + stage * kStage, [](int) {});
+      multiply(lds + at_a * OpA::kBytes, lds + kLdsA + at_b * OpB::kBytes, [](int) {});
       if (s + 1 < steps) {
-        OpA::put(lds + before * kStage, ra);
-        OpB::put(lds + before * kStage + OpA::kBytes, rb);
+        OpA::put(lds + (at_a ^ 1) * OpA::kBytes, ra);
+        OpB::put(lds + kLdsA + (at_b ^ 1) * OpB::kBytes, rb);
       }
     }
-    stage = stage + 1 == kStages ? 0 : stage + 1;
+    at_a = at_a + 1 == kStagesA ? 0 : at_a + 1;
+    at_b = at_b + 1 == kStagesB ? 0 : at_b + 1;
   }
   // (nothing may be on its way into LDS when the workgroup ends)
   if constexpr (kDirect) wait_loads<0>();
@@ -363,7 +373,7 @@ __global__ __launch_bounds__(64 * kWM * kWN, 2) void grouped_tile_kernel(Grouped
   // To the output through LDS, so that a store covers whole lines: each wavefront has a share of the stages for itself,
   // kRows rows of its kCols columns at a time, 16-byte pieces permuted by row.
   constexpr int kCols = kBN / kWN, kPiece = kPer16<TO>, kPieces = kCols / kPiece, kRowBytes = kCols * (int)sizeof(TO);
-  constexpr int kShare = kStages * kStage / (kWM * kWN), kRows = kShare / kRowBytes < kBM / kWM ? kShare / kRowBytes : kBM / kWM;
+  constexpr int kShare = kLds / (kWM * kWN), kRows = whole_rows(kShare / kRowBytes, kBM / kWM);
   static_assert(kRows % 16 == 0 && kBM / kWM % kRows == 0 && kPieces <= 64, "whole fragments and rows");
   __syncthreads();
   char* mine = lds + wave * kShare;

@@ -107,7 +107,7 @@ int sort_rows(hpspmm_rows_plan* plan, int64_t n, int64_t ids, const void* d_ids,
   const int64_t n_offsets = d_offsets ? ids + 1 : 0;
   // Counting ranks costs n^2 / 16 steps of a wavefront in all, digits two dependent launches each: 512 rows 5 us against
   // 12, 8192 rows and 2^17 ids 10 against 20, about the same at 16384.
-  if (n <= kRankMaxRows && (n_offsets <= 4 * kRankMaxRows || n == 0)) {
+  if (n <= kRankMaxRows && n_offsets <= 4 * kRankMaxRows) {
     const int64_t count = n + n_offsets;
     if (count == 0 && zero.rows == 0) return HPSPMM_OK;
     const ZeroFill z = zero.next(ceil_div(count, 64), 1, 64 * kRankWaves, &grid);
@@ -121,6 +121,7 @@ int sort_rows(hpspmm_rows_plan* plan, int64_t n, int64_t ids, const void* d_ids,
   }
   int digits, bits;
   key_digits(ids, &digits, &bits);
+  if (n == 0) digits = 0;
   const int64_t tiles = ceil_div(n, kDigitTile);
   const bool fused = tiles <= kDigitFused;
   // offsets come with the only digit, or from the sorted keys
@@ -144,7 +145,7 @@ int sort_rows(hpspmm_rows_plan* plan, int64_t n, int64_t ids, const void* d_ids,
     });
     if (rc) return rc;
   }
-  const int at = (digits - 1) & 1;
+  const int at = (digits + 1) & 1;
   if (d_offsets && !with_offsets)
     hipLaunchKernelGGL(row_offsets_kernel, dim3((unsigned)ceil_div(n_offsets, kBlock)), dim3(kBlock), 0, st, n, ids,
                        plan->d_keys[at], d_offsets);
@@ -329,7 +330,7 @@ HPSPMM_API int hpspmm_embedding_grad(hpspmm_rows_plan* plan, int64_t n, int64_t 
   const dim3 fix_grid((unsigned)s.chunks, (unsigned)ceil_div(width, 256));
   dispatch_dtype(table_type, [&](auto o) {
     using TO = decltype(o);
-    dispatch_dtype(grad_type, [&](auto t) {
+    if (sum_blocks + zero_blocks > 0) dispatch_dtype(grad_type, [&](auto t) {
       using T = decltype(t);
       auto launch = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)(sum_blocks + zero_blocks), (unsigned)s.col_tiles), dim3(threads), 0, st, g);

@@ -463,7 +463,7 @@ int hpspmm_embedding_lookup(int64_t n, int64_t vocab, int64_t width, const void 
  * (any pair of types).  Without `accumulate` every row of the table is written,
  * zeros where no id points; with it the rows that no id points at are not
  * touched.  The rows of one id are added in an order that depends on the ids
- * alone.
+ * and the sizes alone.
  */
 int hpspmm_embedding_grad(hpspmm_rows_plan *plan, int64_t n, int64_t vocab, int64_t width, const void *d_ids,
                           int id_type, const void *d_grad, int64_t ld_grad, int grad_type, float scale, void *d_table,

@@ -154,10 +154,16 @@ def _grad_reference(ids, grad, vocab, scale):
     torch = _torch()
     here = _in_table(ids, vocab)
     at, x = ids.long()[here], grad[here].double() * float(np.float32(scale))
-    value = torch.zeros(vocab, grad.shape[1], device=grad.device, dtype=torch.float64).index_add_(0, at, x)
-    absolute = torch.zeros_like(value).index_add_(0, at, x.abs())
-    count = torch.zeros(vocab, 1, device=grad.device, dtype=torch.float64).index_add_(
-        0, at, torch.ones(at.shape[0], 1, device=grad.device, dtype=torch.float64))
+
+    def sums(v):
+        out = torch.zeros(vocab, grad.shape[1], device=grad.device, dtype=torch.float64)
+        if at.numel() and bool((at == at[0]).all()):  # (64-bit atomic additions to one row crawl)
+            out[at[0]] = v.sum(0)
+            return out
+        return out.index_add_(0, at, v)
+
+    value, absolute = sums(x), sums(x.abs())
+    count = torch.bincount(at, minlength=vocab)[:, None].double()
     return value, absolute, count
 
 
@@ -192,6 +198,38 @@ def test_lookup_gradient(pkg, gpu, kind, out_kind, layout, how, n, vocab, width)
     assert bool(torch.isnan(base.view[~met]).all())
     base.check_around()
     plan.destroy()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("layout", ["contiguous", "aligned_slice", "odd_slice"])
+@pytest.mark.parametrize("vocab, width", [(1, 1), (300, 129), (5000, 264), (70000, 3)])
+def test_lookup_gradient_of_no_rows(pkg, gpu, kind, layout, vocab, width):
+    torch = _torch()
+    plan = pkg.capi.RowsPlan(0, vocab, width)
+    ids, grad = torch.empty(0, device=gpu, dtype=torch.int64), torch.empty(0, width, device=gpu, dtype=_t(kind))
+    out = Guarded(gpu, (vocab, width), kind, layout)
+    pkg.capi.embedding_grad(plan, ids, grad, out.view, accumulate=True)
+    assert bool(torch.isnan(out.view).all())
+    pkg.capi.embedding_grad(plan, ids, grad, out.view)
+    assert not out.view.any() and not torch_isnan(out.view)
+    out.check_around()
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float32"])
+@pytest.mark.parametrize("width", [512, 777])
+def test_lookup_gradient_of_a_table_larger_than_the_sort_fills(pkg, gpu, kind, width):
+    """More than 192 MB of rows that get a sum: the rows that get none are filled beside the sums instead."""
+    torch = _torch()
+    g = _gen(gpu, 11)
+    n, vocab = 220000, 230000
+    ids = torch.randperm(vocab, device=gpu, generator=g)[:n].to(torch.int32)
+    ids[::7] = -1
+    ids[1::5000] = ids[1]
+    grad = torch.randn(n, width, device=gpu, generator=g).to(_t(kind))
+    out = torch.full((vocab, width), float("nan"), device=gpu, dtype=_t(kind))
+    pkg.capi.embedding_grad(pkg.capi.RowsPlan(n, vocab, width), ids, grad, out)
+    value, absolute, count = _grad_reference(ids, grad, vocab, 1.0)
+    _check(out, value, absolute, count)
 
 
 def test_lookup_gradient_against_differences(pkg, gpu):
@@ -367,6 +405,29 @@ def test_grouped_products_with_offsets_that_are_none(pkg, gpu, kind):
         torch.cuda.synchronize()
         for one in outs:
             one.check_around()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_grouped_products_of_no_rows(pkg, gpu, kind):
+    torch = _torch()
+    capi = pkg.capi
+    x, dy = torch.empty(0, 40, device=gpu, dtype=_t(kind)), torch.empty(0, 24, device=gpu, dtype=_t(kind))
+    w = torch.ones(3, 24, 40, device=gpu, dtype=_t(kind))
+    offsets = torch.zeros(4, dtype=torch.int32, device=gpu)
+    capi.grouped_mm(x, w, offsets, torch.empty_like(dy))
+    capi.grouped_mm_grad_x(dy, w, offsets, torch.empty_like(x))
+    dw = torch.full_like(w, float("nan"))
+    capi.grouped_mm_grad_w(capi.RowsPlan(0, 3), dy, x, offsets, dw)
+    assert not dw.any() and not torch_isnan(dw)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("layout", ["contiguous", "odd_slice"])
+@pytest.mark.parametrize("how", ["ragged", "one"])
+@pytest.mark.parametrize("rows, groups, k, m", [(9000, 2, 200, 89), (5000, 1, 128, 128), (6000, 3, 64, 40)])
+def test_gradients_of_weights_in_parts(pkg, gpu, kind, layout, how, rows, groups, k, m):
+    """Few output tiles and long groups: the rows are cut into parts."""
+    test_grouped_products(pkg, gpu, kind, layout, how, rows, groups, k, m)
 
 
 def test_grouped_product_of_shared_weights(pkg, gpu):
