@@ -122,8 +122,24 @@ struct Operand {
                  : "memory", "m0");
   }
 
-  // The same for rows at any alignment and of any length, through registers.
-  __device__ __forceinline__ void load_loose(Chunk (&regs)[kPer], int64_t left) {
+  // The same for rows at any alignment and of any length, through registers.  Steps from which on chunks would run over
+  // the end of the matrix (the last one, if any); in those before, a chunk that runs over the end of its row reads on into
+  // the next row - what it gives there is not stored -, and no load hangs on a condition, for which it would wait.
+  __device__ __forceinline__ int64_t inner_steps(int64_t depth) const {
+    return kCol && valid < kB && depth > 0 ? (depth - 1) / kDepth : depth / kDepth;
+  }
+  __device__ __forceinline__ void load_inner(Chunk (&regs)[kPer]) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      int r, c;
+      place(i, r, c);
+      if constexpr (kCol) c = min(c, (valid - 1) / kChunk);
+      else r = min(r, valid - 1);
+      regs[i] = *reinterpret_cast<const typename Pack<T, kChunk, false>::type*>((const T*)(base + (int64_t)r * ld) + c * kChunk);
+    }
+    base += step;
+  }
+  __device__ __forceinline__ void load_last(Chunk (&regs)[kPer], int64_t left) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       int r, c;
@@ -131,14 +147,9 @@ struct Operand {
       // elements of the chunk that exist
       const int64_t there = kCol ? (r < left ? (int64_t)valid - c * kChunk : 0) : left - c * kChunk;
       const T* p = (const T*)(base + (int64_t)(kCol ? r : min(r, valid - 1)) * ld) + c * kChunk;
-      if (there >= kChunk) {
-        regs[i] = *reinterpret_cast<const typename Pack<T, kChunk, false>::type*>(p);
-      } else {
 #pragma unroll
-        for (int e = 0; e < kChunk; ++e) regs[i][e] = e < there ? p[e] : (T)0.f;
-      }
+      for (int e = 0; e < kChunk; ++e) regs[i][e] = e < there ? p[e] : (T)0.f;
     }
-    base += step;
   }
   static __device__ __forceinline__ void put(char* lds, const Chunk (&regs)[kPer]) {
 #pragma unroll
@@ -296,8 +307,22 @@ __global__ __launch_bounds__(64 * kWM * kWN, 2) void grouped_tile_kernel(Grouped
   static_assert(kStagesA == kStagesB || kStagesA == kStagesB + 1, "a is asked for after b, and at most a step further ahead");
   static_assert(kDirect || (kStagesA == 2 && kStagesB == 2), "loads through registers are one step ahead");
   const int64_t steps = (depth + kDepth - 1) / kDepth;
-  typename OpA::Chunk ra[kDirect ? 1 : OpA::kPer];
-  typename OpB::Chunk rb[kDirect ? 1 : OpB::kPer];
+  typename OpA::Chunk ra[OpA::kPer];
+  typename OpB::Chunk rb[OpB::kPer];
+  const int64_t inner = kDirect ? 0 : min(a.inner_steps(depth), b.inner_steps(depth));
+  auto load_loose = [&](int64_t s) {
+    if (s < inner) {
+      a.load_inner(ra);
+      b.load_inner(rb);
+    } else {
+      a.load_last(ra, depth - s * kDepth);
+      b.load_last(rb, depth - s * kDepth);
+    }
+  };
+  auto put_loose = [&](int64_t s) {
+    OpA::put(lds + (s & 1) * OpA::kBytes, ra);
+    OpB::put(lds + kLdsA + (s & 1) * OpB::kBytes, rb);
+  };
   const uint32_t lds_wave = (uint32_t)(uintptr_t)(lds_char*)lds + (uint32_t)wave * 1024u;  // where this wavefront's chunks go
   static_assert(FN <= FM, "the fragments of a half are read between the sums of the half before");
   int next_a = 0, next_b = 0;  // steps asked for
@@ -329,34 +354,28 @@ __global__ __launch_bounds__(64 * kWM * kWN, 2) void grouped_tile_kernel(Grouped
 #pragma unroll
       for (int s = 0; s < kStagesA - 1; ++s) ask_both(s >= kStagesA - kStagesB);
     } else {
-      a.load_loose(ra, depth);
-      b.load_loose(rb, depth);
-      OpA::put(lds, ra);
-      OpB::put(lds + kLdsA, rb);
+      load_loose(0);
+      put_loose(0);
     }
   }
-  int at_a = 0, at_b = 0;  // places of the step at hand
-  for (int64_t s = 0; s < steps; ++s) {
-    if constexpr (kDirect) {
+  if constexpr (kDirect) {
+    int at_a = 0, at_b = 0;  // places of the step at hand
+    for (int64_t s = 0; s < steps; ++s) {
       wait_loads<(kStagesA - 2) * OpA::kPer + (kStagesB - 2) * OpB::kPer>();
       meet();
       multiply(lds + at_a * OpA::kBytes, lds + kLdsA + at_b * OpB::kBytes, [&](int i) {
         if (i == 0) ask_both(true);
       });
-    } else {
-      __syncthreads();
-      if (s + 1 < steps) {
-        a.load_loose(ra, depth - (s + 1) * kDepth);
-        b.load_loose(rb, depth - (s + 1) * kDepth);
-      }
-      multiply(lds + at_a * OpA::kBytes, lds + kLdsA + at_b * OpB::kBytes, [](int) {});
-      if (s + 1 < steps) {
-        OpA::put(lds + (at_a ^ 1) * OpA::kBytes, ra);
-        OpB::put(lds + kLdsA + (at_b ^ 1) * OpB::kBytes, rb);
-      }
+      at_a = at_a + 1 == kStagesA ? 0 : at_a + 1;
+      at_b = at_b + 1 == kStagesB ? 0 : at_b + 1;
     }
-    at_a = at_a + 1 == kStagesA ? 0 : at_a + 1;
-    at_b = at_b + 1 == kStagesB ? 0 : at_b + 1;
+  } else {
+    for (int64_t s = 0; s < steps; ++s) {
+      __syncthreads();
+      if (s + 1 < steps) load_loose(s + 1);
+      multiply(lds + (s & 1) * OpA::kBytes, lds + kLdsA + (s & 1) * OpB::kBytes, [](int) {});
+      if (s + 1 < steps) put_loose(s + 1);
+    }
   }
   // (nothing may be on its way into LDS when the workgroup ends)
   if constexpr (kDirect) wait_loads<0>();
