@@ -167,6 +167,7 @@ SumShape sum_shape(int64_t n, int64_t width, int64_t per16) {
   // chunks as long as leaves 1024 of them a column tile, at most 128 rows
   s.chunk_log2 = kMinChunkLog2;
   while (s.chunk_log2 < kMaxChunkLog2 && (n * s.col_tiles) >> (s.chunk_log2 + 1) >= 1024) ++s.chunk_log2;
+  if (n <= 32) s.chunk_log2 = 5;  // one chunk: no sum crosses it, one launch less
   s.chunks = ceil_div(n, (int64_t)1 << s.chunk_log2);
   s.pitch = ceil_div(width, 8) * 8;
   return s;
