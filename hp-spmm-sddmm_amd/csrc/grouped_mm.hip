@@ -48,20 +48,22 @@ int64_t expected_tiles(int mode, const hpspmm::GroupedArgs& g, int64_t edge) {
   return cols * std::max<int64_t>(1, std::min(g.rows, g.rows / edge + g.groups / 2));
 }
 
-// Edge of the output tiles, 256 (16-bit operands at multiples of 16 bytes), 128 or 64: rate of the tile times the share
-// of the chip that the last round of tiles leaves busy.  Rates of 16-bit products of 32768 x 2048 x 4096 over 32 groups:
-// 950, 800 and 500 TFLOP/s; a CU holds 1, 2 and 2 of the workgroups.  bf16, rows x groups x k x m, 64 / 128 / 256 in us:
-// 2000 x 8 x 1024 x 1024 16 / 16 / 32, 8192 x 8 x 1024 x 1024 41 / 34 / 34, 8192 x 8 x 2048 x 2048 119 / 89 / 109.
-int tile_edge(int mode, const hpspmm::GroupedArgs& g, bool large) {
-  const struct { int edge; int64_t slots; double rate; } kinds[] = {{256, 256, 9.5}, {128, 512, 8.0}, {64, 512, 5.0}};
+// Edge of the output tiles, 256 (16-bit operands at multiples of 16 bytes), 128 or 64: the one that is expected to take
+// the least time, tiles per CU (one at least, and a part of a round that is not full) times the area of a tile over its
+// rate.  bf16, rows x groups x k x m, product with tiles of 64 / 128 / 256 in us: 32768 x 32 x 2048 x 4096 933 / 588 / 526
+// (the rates), 8192 x 8 x 2048 x 2048 113 / 76 / 99, 8192 x 8 x 1024 x 1024 39 / 28 / 30, 2000 x 8 x 1024 x 1024 15 / 13 /
+// 28, 32 x 64 x 2048 x 1024 18 / 24 / 46 (the last two set the rate of 64, which is 580 TFLOP/s in the first).  32-bit
+// products wait for the matrix cores whatever the tile: 1777 x 10 x 1001 x 519, gradient of x 27 / 47 us.
+int tile_edge(int mode, const hpspmm::GroupedArgs& g, bool wide, bool large) {
+  const struct { int edge; double rate; } kinds[] = {{256, 1030}, {128, 920}, {64, wide ? 800 : 490}};
   int best = 64;
-  double most = 0;
+  double least = 0;
   for (const auto& q : kinds) {
     if (q.edge == 256 && !large) continue;
-    const int64_t tiles = expected_tiles(mode, g, q.edge);
-    const double score = q.rate * (double)tiles / (double)(ceil_div(tiles, q.slots) * q.slots);
-    if (score > most) {
-      most = score;
+    const double per_cu = std::max(1.0, (double)expected_tiles(mode, g, q.edge) / 256 + 0.3);
+    const double time = per_cu * q.edge * q.edge / q.rate;
+    if (least == 0 || time < least) {
+      least = time;
       best = q.edge;
     }
   }
@@ -83,6 +85,7 @@ int launch_tiles(const hpspmm::GroupedArgs& g, hipStream_t st) {
 
 // Parts that the rows of every group are cut into for the gradient of the weights, 1 = none: where there are few output
 // tiles and long groups, as many as give every slot of the chip a tile, each of at least 4 steps of the mean group.
+// 18867 x 2 x 2304 x 89 bf16 131 -> 41 us, 32768 x 1 x 512 x 512 131 -> 30 us, 9000 x 2 x 200 x 89 34 -> 18 us.
 int row_splits(const hpspmm::GroupedArgs& g, int64_t depth) {
   const int64_t tiles = expected_tiles(hpspmm::kGradW, g, hpspmm::kSplitEdge);
   const int64_t steps = g.rows / g.groups / depth;
@@ -122,7 +125,7 @@ int launch_grouped(const hpspmm::GroupedArgs& g, int dtype, int out_type, hipStr
           const int splits = row_splits(g, 128 / (int64_t)sizeof(T));
           if (splits > 1) return launch_split<T, TO>(g, splits, direct, st);
         }
-        const int edge = tile_edge(kMode, g, sizeof(T) == 2 && direct);
+        const int edge = tile_edge(kMode, g, sizeof(T) == 4, sizeof(T) == 2 && direct);
         if constexpr (sizeof(T) == 2) {
           if (edge == 256) return launch_tiles<T, TO, kMode, 256, 256, 2, 4, true, 8, 3, 2>(g, st);
         }

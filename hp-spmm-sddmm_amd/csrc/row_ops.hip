@@ -105,23 +105,32 @@ int sort_rows(hpspmm_rows_plan* plan, int64_t n, int64_t ids, const void* d_ids,
   unsigned grid = 0;
   if (out) *out = {plan->d_keys[0], plan->d_vals[0]};
   const int64_t n_offsets = d_offsets ? ids + 1 : 0;
-  // Counting ranks costs n^2 / 16 steps of a wavefront in all, digits two dependent launches each: 512 rows 5 us against
-  // 12, 8192 rows and 2^17 ids 10 against 20, about the same at 16384.
-  if (n <= kRankMaxRows && n_offsets <= 4 * kRankMaxRows) {
-    const int64_t count = n + n_offsets;
-    if (count == 0 && zero.rows == 0) return HPSPMM_OK;
-    const ZeroFill z = zero.next(ceil_div(count, 64), 1, 64 * kRankWaves, &grid);
-    return dispatch_id(id_type, [&](auto id) {
-      using Id = decltype(id);
-      hipLaunchKernelGGL((row_rank_kernel<Id>), dim3(grid), dim3(64 * kRankWaves), 0, st, (int32_t)n,
-                         (int32_t)n_offsets, (uint32_t)ids, (const Id*)d_ids, d_order ? nullptr : plan->d_keys[0],
-                         d_order ? d_order : plan->d_vals[0], d_offsets, z);
-      return HPSPMM_OK;
-    });
-  }
+  auto offsets_of = [&](const uint32_t* keys) {
+    hipLaunchKernelGGL(row_offsets_kernel, dim3((unsigned)ceil_div(n_offsets, kBlock)), dim3(kBlock), 0, st, n, ids, keys,
+                       d_offsets);
+  };
   int digits, bits;
   key_digits(ids, &digits, &bits);
-  if (n == 0) digits = 0;
+  // Counting ranks is one launch of n^2 steps, digits are two dependent launches each.  64 ids (one digit), ranks / digits:
+  // 4096 rows 7.9 / 9.9 us, 8192 rows 13.0 / 10.4; 131072 ids (two digits), with the sums of a gradient behind them: 512
+  // rows 12 / 24 us, 8192 rows 28 / 41, 16384 rows 46 / 48.
+  if (n <= (digits == 1 ? 6144 : kRankMaxRows)) {
+    // few groups are counted along as if they were rows, many found in the sorted keys
+    const bool counted = n_offsets <= 4 * kRankMaxRows;
+    const int64_t count = n + (counted ? n_offsets : 0);
+    if (count > 0 || zero.rows > 0) {
+      const ZeroFill z = zero.next(ceil_div(count, 64), 1, 64 * kRankWaves, &grid);
+      dispatch_id(id_type, [&](auto id) {
+        using Id = decltype(id);
+        hipLaunchKernelGGL((row_rank_kernel<Id>), dim3(grid), dim3(64 * kRankWaves), 0, st, (int32_t)n,
+                           counted ? (int32_t)n_offsets : 0, (uint32_t)ids, (const Id*)d_ids,
+                           d_order && counted ? nullptr : plan->d_keys[0], d_order ? d_order : plan->d_vals[0], d_offsets, z);
+        return HPSPMM_OK;
+      });
+    }
+    if (!counted) offsets_of(plan->d_keys[0]);
+    return HPSPMM_OK;
+  }
   const int64_t tiles = ceil_div(n, kDigitTile);
   const bool fused = tiles <= kDigitFused;
   // offsets come with the only digit, or from the sorted keys
@@ -146,9 +155,7 @@ int sort_rows(hpspmm_rows_plan* plan, int64_t n, int64_t ids, const void* d_ids,
     if (rc) return rc;
   }
   const int at = (digits + 1) & 1;
-  if (d_offsets && !with_offsets)
-    hipLaunchKernelGGL(row_offsets_kernel, dim3((unsigned)ceil_div(n_offsets, kBlock)), dim3(kBlock), 0, st, n, ids,
-                       plan->d_keys[at], d_offsets);
+  if (d_offsets && !with_offsets) offsets_of(plan->d_keys[at]);
   if (out) *out = {plan->d_keys[at], plan->d_vals[at]};
   return HPSPMM_OK;
 }
@@ -311,9 +318,10 @@ HPSPMM_API int hpspmm_embedding_grad(hpspmm_rows_plan* plan, int64_t n, int64_t 
   hipStream_t st = (hipStream_t)stream;
   const int64_t grad_size = dtype_size(grad_type), table_size = dtype_size(table_type);
   // Rows that no id points at become zeros either in the launches of the sort, which leave most of the chip idle but know
-  // of no row yet (so every row is filled), or beside the sums, where those that get one are left out.  The first hides
-  // the sort behind the fill, 20 to 40 us, and writes at most min(n, vocab) rows twice.
-  const bool early = !accumulate && std::min(n, vocab) * width * table_size <= (int64_t)192 << 20;
+  // of no row yet (so every row is filled), or beside the sums, where the rows that get one are left out.  The first hides
+  // the sort behind the fill and writes the rows that get a sum twice.  Early / late: 1000 ids, 50001 x 771 f32 28 / 36 us,
+  // 32768 ids, 131072 x 2048 bf16 161 / 178 us, 262144 ids, 32768 x 1024 f32 208 / 196 us.
+  const bool early = !accumulate && n <= vocab && n * width * table_size <= (int64_t)192 << 20;
   const ZeroRows zero = early ? ZeroRows(d_table, vocab, width * table_size, ld_table * table_size) : ZeroRows();
   Sorted sorted{};
   if (int rc = sort_rows(plan, n, vocab, d_ids, id_type, nullptr, nullptr, zero, st, &sorted)) return rc;

@@ -284,7 +284,7 @@ def test_plan_limits_are_kept(pkg, gpu):
 @pytest.mark.parametrize("id_kind", ["int32", "int64"])
 @pytest.mark.parametrize("how", ["mixed", "one", "none"])
 @pytest.mark.parametrize("n, groups", [(0, 4), (1, 1), (5, 300), (64, 8), (1000, 7), (2048, 64), (2049, 1000), (8192, 16),
-                                       (8193, 5000), (40000, 255), (70000, 256), (70000, 257), (300001, 130), (5000, 1 << 20), (600001, 300),
+                                       (8193, 5000), (40000, 255), (70000, 256), (70000, 257), (300001, 130), (5000, 1 << 20), (600001, 300), (6144, 1000), (6145, 1000), (16384, 5000), (16385, 5000), (3000, 70000),
                                        (1100000, 5000)])
 def test_group_rows(pkg, gpu, id_kind, how, n, groups):
     torch = _torch()
