@@ -55,7 +55,7 @@ int64_t expected_tiles(int mode, const hpspmm::GroupedArgs& g, int64_t edge) {
 // 28, 32 x 64 x 2048 x 1024 18 / 24 / 46 (the last two set the rate of 64, which is 580 TFLOP/s in the first).  32-bit
 // products wait for the matrix cores whatever the tile: 1777 x 10 x 1001 x 519, gradient of x 27 / 47 us.
 int tile_edge(int mode, const hpspmm::GroupedArgs& g, bool wide, bool large) {
-  const struct { int edge; double rate; } kinds[] = {{256, 1030}, {128, 920}, {64, wide ? 800 : 490}};
+  const struct { int edge; double rate; } kinds[] = {{256, 1030}, {128, 920}, {64, wide ? 800.0 : 490.0}};
   int best = 64;
   double least = 0;
   for (const auto& q : kinds) {
