@@ -12,6 +12,15 @@
 //
 // Rows beyond the group and columns beyond the matrix repeat the last one that exists - what they give is not stored;
 // terms beyond the contraction are zeros in both operands, whatever lies there in memory.
+//
+// Sums are held in 32 bits by the matrix instructions (16 x 16 x 32 for 16-bit, 16 x 16 x 4 for 32-bit elements) and
+// rounded once.  bf16, 32768 rows, 32 groups, k 2048, m 4096, tiles of 256: product 526 us (1029 TFLOP/s), gradient of x
+// 522 us, of w in 32 bits 699 us; the matrix cores are busy 55, 58 and 44 % of the time, an eighth of it with rows beyond
+// the ends of groups.  What bounds it is the way of the operands into LDS: without the products the same loads take 510 us,
+// without the loads the products 405 us; a CU has about 64 lines under way, at 570 cycles each (a larger tile, fewer
+// bytes, does not fit 160 KB of LDS).  Reads of LDS meet no bank conflicts in any of the three.  On the way: loads with
+// the builtin, whose counter every transposed read waits for, 715 / 944 us for the gradients; steps of 32 terms, half a
+// line a row, 650 / 870 / 1155 us; tiles in rows instead of panels, a third more requests to memory, 575 instead of 562 us.
 #pragma once
 
 #include "grouped_kernels.hpp"

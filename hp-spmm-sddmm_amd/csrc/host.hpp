@@ -13,6 +13,8 @@
 //   plan_sweep.hip     sweep layout             launch_sweep.hip    its kernels' launches
 //   launch_rows.hip    whole rows: CSR arrays, row tiles, run-time row lengths
 //   launch_segments.hip  segments (+ hub cache), ordered, COO accumulate, static workspace
+//   row_ops.hip        rows selected by an id: embedding lookup and its gradient, rows sorted by id, their plan
+//   grouped_mm.hip     products grouped by expert (both: row_ops.hpp)
 #pragma once
 
 #include "hpspmm.h"

@@ -6,9 +6,12 @@
 
 namespace hpspmm {
 
-// out[i, :] = scale * table[ids[i], :], rows of zeros for ids outside the table.  A thread owns 16 bytes of a row;
-// 2^tpr_log2 adjacent threads share a row's column tile, a workgroup covers kRows rows one after the other, all of
-// whose loads are in flight together.
+// out[i, :] = scale * table[ids[i], :], rows of zeros for ids outside the table: one product in 32 bits, rounded once.
+// Bound by the bytes, n rows read and n written.  A thread owns 16 bytes of a row; 2^tpr_log2 adjacent threads share a
+// row's column tile, a workgroup covers kRows rows one after the other, all of whose loads are in flight together.
+// kStream: large outputs go past the caches, which they do not fit (32768 rows of 4096 bf16 over 131072: 84 -> 63 us with
+// the table's rows partly in the caches; 82 us = 4.5 TB/s of distinct rows and output where they are not).  16 rows of
+// 1024 take 7 us from Python, half of it the launch.
 template <class T, class Id, bool kAligned, int kRows, bool kStream>
 __global__ __launch_bounds__(kBlock) void embedding_lookup_kernel(int64_t n, uint32_t vocab, int32_t width, int tpr_log2,
                                                                  const Id* __restrict__ ids, const T* __restrict__ table,
@@ -59,7 +62,7 @@ __global__ __launch_bounds__(kBlock) void embedding_lookup_kernel(int64_t n, uin
 
 // Rows of zeros, for the launches that have workgroups to spare: rows [0, rows) of `bytes` bytes (the last one of
 // `last`), `pitch` bytes apart, by `blocks` workgroups from workgroup `first` on, 2^tpr_log2 threads a row.  An all-zero
-// word is a zero of every element type.
+// word is a zero of every element type.  A quarter of 131072 x 2048 bf16 with each launch of a sort: 21 us, 6.4 TB/s.
 struct ZeroFill {
   char* at;
   int64_t rows, bytes, last, pitch;
@@ -114,7 +117,7 @@ HPSPMM_KERNEL __launch_bounds__(kBlock) void row_offsets_kernel(int64_t n, int64
 }
 
 // Few rows: the place of a row is the number of rows before it, counted - n^2 comparisons, but one launch and no step
-// that waits for another.  A workgroup places 64 rows, one a lane; its 16 wavefronts count in a sixteenth of the rows
+// that waits for another (512 rows, 16 groups: 4 us on the device).  Bound by the comparisons, 2 instructions each.  A workgroup places 64 rows, one a lane; its 16 wavefronts count in a sixteenth of the rows
 // each, which they hold in LDS.  Rows n ... n + virtual - 1 are the group numbers 0 ...: their place is their offset.
 constexpr int kRankWaves = 16;
 constexpr int kRankMaxRows = 16384;
@@ -182,7 +185,9 @@ __global__ __launch_bounds__(64 * kRankWaves) void row_rank_kernel(int32_t n, in
 
 // Many rows: stable counting sort by digits of up to 10 bits, least significant first, two launches a digit: counts per
 // tile of rows, then the rows to their places.  A tile's rows go to the wavefronts in stretches of 4 x 64; a row's rank
-// among the equal digits of its stretch is found by ballots over the digit's bits.
+// among the equal digits of its stretch is found by ballots over the digit's bits.  Bound by the chain of its steps: keys,
+// counts of the other tiles, places, rows.  524288 rows, 64 groups: 3 + 10 us, 0.5 TB/s (three kernels a digit of 8 bits,
+// with a scan between counts and places: 37 us).  Ten bits a digit let 2^20 ids do with two.
 constexpr int kDigitBits = 10, kDigitBins = 1 << kDigitBits;
 constexpr int kDigitThreads = 1024, kDigitWaves = kDigitThreads / 64, kDigitRounds = 4;
 constexpr int kDigitTile = kDigitThreads * kDigitRounds;
@@ -329,10 +334,16 @@ __global__ __launch_bounds__(kDigitThreads) void digit_scatter_kernel(int64_t n,
 // Gradient of the lookup: sums over the stretches of equal keys of the sorted rows.  A chunk of 2^chunk_log2 sorted rows
 // is added up by one group of threads, 16 bytes of a row each; a sum that lies within the chunk goes to the table, one
 // that began before it to carry slot 2c, one that goes on behind it to slot 2c + 1 (32 bits), and a second kernel adds
-// those up in order.  No atomics: the same ids give the same bits.
+// those up in order.  No atomics: the same ids give the same bits.  Sums are held in 32 bits and rounded once.
+//
+// Bound by the bytes: rows of the gradient in a random order, rows of the table written.  262144 rows of 1024 bf16 over
+// 32768 rows of f32: 537 + 134 MB in 150 us, 4.5 TB/s (an addition over all of a large array reads at 4.0); one workgroup
+// for each row of the table that walks its rows: 4300 us, the frequent ids being one chain.  Chunks of 16 to 128 rows:
+// the fewer, the less is carried (32768 rows of 2048, 16 / 32 / 64 rows a chunk: 165 / 161 / 160 us in all).  16 instead
+// of 8 rows in flight: fewer workgroups on a CU, 268 -> 380 us.
 // ---------------------------------------------------------------------------------------------
 
-constexpr int kSumFlight = 8;  // rows in flight
+constexpr int kSumFlight = 8;  // rows in flight (4: the same times)
 
 // Sorted keys and rows, as the kernel finds them: reads at addresses that a whole workgroup shares go through scalar
 // registers.
@@ -478,8 +489,10 @@ __global__ __launch_bounds__(kBlock) void embedding_sum_kernel(SumArgs g) {
   close(open ? 0 : goes_on ? 1 : -1);
 }
 
-// The sums that cross chunks: the chunk in which one begins adds up its slots.  One workgroup per chunk and 256 columns;
-// its wavefronts take a stretch of the slots each, and their sums are added in that order.
+// The sums that cross chunks: the chunk in which one begins adds up its slots.  One workgroup per chunk and 256 columns
+// (most have nothing to do); its wavefronts take a stretch of the slots each, and their sums are added in that order.
+// Bound by its chain of loads, 3 to 11 us: keys around the chunk's end, keys at the starts of the next 64 chunks, slots.
+// (Workgroups that looked at 8 chunks each and searched for a sum's end: 41 to 48 us.)
 template <class TO, bool kWhole>
 __global__ __launch_bounds__(kBlock) void embedding_fix_kernel(SumArgs g) {
   __shared__ float s_part[kWavesPerBlock][64][4];

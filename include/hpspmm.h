@@ -438,7 +438,8 @@ typedef enum hpspmm_id_type { HPSPMM_I32 = 0, HPSPMM_I64 = 1 } hpspmm_id_type;
 /*
  * Workspace of the row operators that sort or split, made once for the largest
  * sizes to come and kept: rows, ids (vocabulary or groups) and columns per row
- * (0 where hpspmm_embedding_grad is not called).  It lives on the device that
+ * (0 where hpspmm_embedding_grad is not called); 32 MB of it, whatever the
+ * sizes, are for the sums that hpspmm_grouped_mm_grad_w splits.  It lives on the device that
  * is current here and is used from one stream at a time; two captured graphs
  * that use the same plan must not run at the same time.
  */
