@@ -120,7 +120,7 @@ struct Operand {
   // Brings this thread's i-th chunk of a step into LDS without passing registers: a wavefront's 64 chunks land one behind
   // the other.  (Written out: behind the builtin the compiler lets every transposed read of LDS wait for all loads that
   // are under way.  The load has no output register; wait_loads() waits
-  // for it.  One wait state lies between the write of m0 and its use.)
+  // for it.  One wait state lies between the write of m0 and its use; nothing else in the kernel uses m0.)
   __device__ __forceinline__ void load_direct(uint32_t lds, int i) const {
     typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
     const uint64_t at = (uint64_t)base;
@@ -128,7 +128,7 @@ struct Operand {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :
                  : "s"(lds + i * kThreads * 16), "v"(offset[i]), "s"(rsrc)
-                 : "memory", "m0");
+                 : "memory");
   }
 
   // The same for rows at any alignment and of any length, through registers.  Steps from which on chunks would run over
