@@ -52,7 +52,8 @@ int64_t expected_tiles(int mode, const hpspmm::GroupedArgs& g, int64_t edge) {
 // the least time, tiles per CU (one at least, and a part of a round that is not full) times the area of a tile over its
 // rate.  bf16, rows x groups x k x m, product with tiles of 64 / 128 / 256 in us: 32768 x 32 x 2048 x 4096 933 / 588 / 526
 // (the rates), 8192 x 8 x 2048 x 2048 113 / 76 / 99, 8192 x 8 x 1024 x 1024 39 / 28 / 30, 2000 x 8 x 1024 x 1024 15 / 13 /
-// 28, 32 x 64 x 2048 x 1024 18 / 24 / 46 (the last two set the rate of 64, which is 580 TFLOP/s in the first).  32-bit
+// 28, 32 x 64 x 2048 x 1024 18 / 24 / 46 (the last two set the rate of 64, which is 580 TFLOP/s in the first); gradient of x
+// of 16384 x 16 x 2048 x 4096, 2.25 rounds of 256, - / 306 / 292.  32-bit
 // products wait for the matrix cores whatever the tile: 1777 x 10 x 1001 x 519, gradient of x 27 / 47 us.
 int tile_edge(int mode, const hpspmm::GroupedArgs& g, bool wide, bool large) {
   const struct { int edge; double rate; } kinds[] = {{256, 1030}, {128, 920}, {64, wide ? 800.0 : 490.0}};
@@ -60,7 +61,7 @@ int tile_edge(int mode, const hpspmm::GroupedArgs& g, bool wide, bool large) {
   double least = 0;
   for (const auto& q : kinds) {
     if (q.edge == 256 && !large) continue;
-    const double per_cu = std::max(1.0, (double)expected_tiles(mode, g, q.edge) / 256 + 0.3);
+    const double per_cu = std::max(1.0, (double)expected_tiles(mode, g, q.edge) / 256 + 0.1);
     const double time = per_cu * q.edge * q.edge / q.rate;
     if (least == 0 || time < least) {
       least = time;

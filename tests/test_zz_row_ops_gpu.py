@@ -410,6 +410,29 @@ def test_grouped_products_with_offsets_that_are_none(pkg, gpu, kind):
             one.check_around()
 
 
+@pytest.mark.parametrize("how", ["ragged", "even", "one"])
+@pytest.mark.parametrize("rows, groups, k, m", [(900, 255, 24, 40), (700, 257, 33, 16), (3000, 1000, 16, 24)])
+def test_grouped_products_of_many_groups(pkg, gpu, how, rows, groups, k, m):
+    torch = _torch()
+    x, dy, w, off, offsets, free = _experts(gpu, groups, rows, groups, k, m, "bfloat16", "contiguous", how)
+    y, dx = torch.full((rows, m), 5.0, device=gpu).bfloat16(), torch.full((rows, k), 5.0, device=gpu).bfloat16()
+    pkg.capi.grouped_mm(x, w, offsets, y)
+    pkg.capi.grouped_mm_grad_x(dy, w, offsets, dx)
+    dw = pkg.capi.grouped_mm_grad_w(pkg.capi.RowsPlan(0, 0), dy, x, offsets, torch.full_like(w, float("nan")))
+    # group of every row, -1 for rows of none
+    sizes = torch.from_numpy(np.diff(off)).to(gpu)
+    of = torch.full((rows,), -1, device=gpu)
+    of[int(off[0]):int(off[-1])] = torch.repeat_interleave(torch.arange(groups, device=gpu), sizes)
+    mine = torch.nonzero(of >= 0).flatten()
+    xe, de, we = x[mine].double(), dy[mine].double(), w[of[mine]].double()
+    _check(y[mine], (we * xe[:, None, :]).sum(2), (we * xe[:, None, :]).abs().sum(2), k)
+    _check(dx[mine], (we * de[:, :, None]).sum(1), (we * de[:, :, None]).abs().sum(1), m)
+    outer = de[:, :, None] * xe[:, None, :]
+    zero = torch.zeros(groups, m, k, device=gpu, dtype=torch.float64)
+    _check(dw, zero.index_add(0, of[mine], outer), zero.index_add(0, of[mine], outer.abs()), sizes[:, None, None].double())
+    assert bool((y[free] == 5.0).all()) and bool((dx[free] == 5.0).all())
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_grouped_products_of_no_rows(pkg, gpu, kind):
     torch = _torch()
