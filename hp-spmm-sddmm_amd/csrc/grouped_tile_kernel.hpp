@@ -119,8 +119,8 @@ struct Operand {
   }
   // Brings this thread's i-th chunk of a step into LDS without passing registers: a wavefront's 64 chunks land one behind
   // the other.  (Written out: behind the builtin the compiler lets every transposed read of LDS wait for all loads that
-  // are under way.  The load has no output register; wait_loads() waits
-  // for it.  One wait state lies between the write of m0 and its use; nothing else in the kernel uses m0.)
+  // are under way.  The load has no output register; wait_loads() waits for it.  One wait state lies between the write of
+  // m0 and its use; nothing else in the kernel uses m0.)
   __device__ __forceinline__ void load_direct(uint32_t lds, int i) const {
     typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
     const uint64_t at = (uint64_t)base;
@@ -131,11 +131,14 @@ struct Operand {
                  : "memory");
   }
 
-  // The same for rows at any alignment and of any length, through registers.  Steps from which on chunks would run over
-  // the end of the matrix (the last one, if any); in those before, a chunk that runs over the end of its row reads on into
-  // the next row - what it gives there is not stored -, and no load hangs on a condition, for which it would wait.
+  // The same for rows at any alignment and of any length, through registers.  Inner steps are those whose chunks stay
+  // within the matrix: there a chunk that runs over the end of its row reads on into the next rows - what it gives is not
+  // stored -, and no load hangs on a condition, for which it would wait.  The one or two steps behind them go by elements.
   __device__ __forceinline__ int64_t inner_steps(int64_t depth) const {
-    return kCol && valid < kB && depth > 0 ? (depth - 1) / kDepth : depth / kDepth;
+    if constexpr (!kCol) return depth / kDepth;
+    // bytes that the last chunk of a row runs over its end, and the rows that they reach into
+    const int64_t over = (int64_t)(((valid - 1) / kChunk + 1) * kChunk - valid) * kSize;
+    return max(depth - (over + ld - 1) / ld, (int64_t)0) / kDepth;
   }
   __device__ __forceinline__ void load_inner(Chunk (&regs)[kPer]) {
 #pragma unroll
@@ -159,6 +162,7 @@ struct Operand {
 #pragma unroll
       for (int e = 0; e < kChunk; ++e) regs[i][e] = e < there ? p[e] : (T)0.f;
     }
+    base += step;
   }
   static __device__ __forceinline__ void put(char* lds, const Chunk (&regs)[kPer]) {
 #pragma unroll

@@ -410,6 +410,15 @@ def test_grouped_products_with_offsets_that_are_none(pkg, gpu, kind):
             one.check_around()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows, groups, k, m", [(65, 1, 1, 1), (66, 1, 1, 3), (70, 1, 2, 130), (129, 1, 3, 1), (200, 2, 1, 70),
+                                                (300, 2, 129, 5), (131, 1, 5, 67)])
+def test_grouped_products_of_narrow_rows(pkg, gpu, kind, rows, groups, k, m):
+    """Rows shorter than 16 bytes, contractions that end just behind a step: the last piece of a row reaches into several
+    rows behind it, and must not do so at the end of the matrix."""
+    test_grouped_products(pkg, gpu, kind, "contiguous", "even", rows, groups, k, m)
+
+
 @pytest.mark.parametrize("how", ["ragged", "even", "one"])
 @pytest.mark.parametrize("rows, groups, k, m", [(900, 255, 24, 40), (700, 257, 33, 16), (3000, 1000, 16, 24)])
 def test_grouped_products_of_many_groups(pkg, gpu, how, rows, groups, k, m):
