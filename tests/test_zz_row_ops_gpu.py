@@ -411,6 +411,27 @@ def test_grouped_products_with_offsets_that_are_none(pkg, gpu, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("layout", ["contiguous", "odd_slice"])
+@pytest.mark.parametrize("rows, groups, k, m", [(300, 5, 129, 65), (9000, 2, 200, 89), (2000, 8, 512, 1024), (2000, 16, 1024, 1024)])
+def test_gradient_of_weights_added_in_their_type(pkg, gpu, kind, layout, rows, groups, k, m):
+    """In tiles of every size and in parts: added to what is there before the one rounding; groups without rows stay."""
+    torch = _torch()
+    x, dy, w, off, offsets, _ = _experts(gpu, rows + m, rows, groups, k, m, kind, layout, "ragged")
+    start = torch.randn(groups, m, k, device=gpu, generator=_gen(gpu, 12)).to(_t(kind))
+    out = Guarded(gpu, (groups, m, k), kind, layout)
+    out.view.copy_(start)
+    pkg.capi.grouped_mm_grad_w(pkg.capi.RowsPlan(0, 0), dy, x, offsets, out.view, accumulate=True)
+    for e in range(groups):
+        r = slice(int(off[e]), int(off[e + 1]))
+        xe, de, base = x[r].double(), dy[r].double(), start[e].double()
+        _check(out.view[e], de.t().contiguous() @ xe + base, de.abs().t().contiguous() @ xe.abs() + base.abs(),
+               r.stop - r.start + 1, f"group {e}")
+        if r.stop == r.start:
+            assert torch.equal(out.view[e], start[e])
+    out.check_around()
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("rows, groups, k, m", [(65, 1, 1, 1), (66, 1, 1, 3), (70, 1, 2, 130), (129, 1, 3, 1), (200, 2, 1, 70),
                                                 (300, 2, 129, 5), (131, 1, 5, 67)])
 def test_grouped_products_of_narrow_rows(pkg, gpu, kind, rows, groups, k, m):
