@@ -71,7 +71,7 @@ int tile_edge(int mode, const hpspmm::GroupedArgs& g, bool wide, bool large) {
   return best;
 }
 
-template <class T, class TO, int kMode, int kBM, int kBN, int kWM, int kWN, bool kDirect, int kC, int kStagesA, int kStagesB>
+template <class T, class TO, int kMode, int kBM, int kBN, int kWM, int kWN, bool kDirect, int kStagesA, int kStagesB>
 int launch_tiles(const hpspmm::GroupedArgs& g, hipStream_t st) {
   const int64_t n_out = kMode == hpspmm::kForward ? g.m : g.k;
   const int64_t col_tiles = ceil_div(n_out, kBN);
@@ -79,7 +79,7 @@ int launch_tiles(const hpspmm::GroupedArgs& g, hipStream_t st) {
   const int64_t tiles = ceil_div(row_tiles * col_tiles, hpspmm::kXcds) * hpspmm::kXcds;
   if (tiles == 0) return HPSPMM_OK;
   if (tiles > INT32_MAX / (64 * kWM * kWN)) return fail(HPSPMM_ERR_INVALID_ARG, "the product has too many output tiles");
-  hipLaunchKernelGGL((hpspmm::grouped_tile_kernel<T, TO, kMode, kBM, kBN, kWM, kWN, kDirect, kC, kStagesA, kStagesB>), dim3((unsigned)tiles),
+  hipLaunchKernelGGL((hpspmm::grouped_tile_kernel<T, TO, kMode, kBM, kBN, kWM, kWN, kDirect, kStagesA, kStagesB>), dim3((unsigned)tiles),
                      dim3(64 * kWM * kWN), 0, st, g, (int)col_tiles);
   return HPSPMM_OK;
 }
@@ -101,10 +101,10 @@ int launch_split(hpspmm::GroupedArgs g, int splits, bool direct, hipStream_t st)
   const int64_t col_tiles = ceil_div(g.k, E), tiles = g.groups * ceil_div(g.m, E) * col_tiles;
   const unsigned grid = (unsigned)(ceil_div(tiles * splits, hpspmm::kXcds) * hpspmm::kXcds);
   if (direct)
-    hipLaunchKernelGGL((hpspmm::grouped_tile_kernel<T, TO, hpspmm::kGradW, E, E, 2, 2, true, 8, 3, 2, true>), dim3(grid), dim3(256), 0,
+    hipLaunchKernelGGL((hpspmm::grouped_tile_kernel<T, TO, hpspmm::kGradW, E, E, 2, 2, true, 3, 2, true>), dim3(grid), dim3(256), 0,
                        st, g, (int)col_tiles);
   else
-    hipLaunchKernelGGL((hpspmm::grouped_tile_kernel<T, TO, hpspmm::kGradW, E, E, 2, 2, false, 8, 2, 2, true>), dim3(grid), dim3(256), 0,
+    hipLaunchKernelGGL((hpspmm::grouped_tile_kernel<T, TO, hpspmm::kGradW, E, E, 2, 2, false, 2, 2, true>), dim3(grid), dim3(256), 0,
                        st, g, (int)col_tiles);
   hipLaunchKernelGGL((hpspmm::grouped_join_kernel<TO>), dim3((unsigned)tiles, E * E / (4 * hpspmm::kBlock)), dim3(hpspmm::kBlock), 0, st,
                      g, (int)col_tiles);
@@ -128,13 +128,13 @@ int launch_grouped(const hpspmm::GroupedArgs& g, int dtype, int out_type, hipStr
         }
         const int edge = tile_edge(kMode, g, sizeof(T) == 4, sizeof(T) == 2 && direct);
         if constexpr (sizeof(T) == 2) {
-          if (edge == 256) return launch_tiles<T, TO, kMode, 256, 256, 2, 4, true, 8, 3, 2>(g, st);
+          if (edge == 256) return launch_tiles<T, TO, kMode, 256, 256, 2, 4, true, 3, 2>(g, st);
         }
         if (edge == 128)
-          return direct ? launch_tiles<T, TO, kMode, 128, 128, 2, 2, true, 8, 3, 2>(g, st)
-                        : launch_tiles<T, TO, kMode, 128, 128, 2, 2, false, 8, 2, 2>(g, st);
-        return direct ? launch_tiles<T, TO, kMode, 64, 64, 2, 2, true, 8, 4, 4>(g, st)
-                      : launch_tiles<T, TO, kMode, 64, 64, 2, 2, false, 8, 2, 2>(g, st);
+          return direct ? launch_tiles<T, TO, kMode, 128, 128, 2, 2, true, 3, 2>(g, st)
+                        : launch_tiles<T, TO, kMode, 128, 128, 2, 2, false, 2, 2>(g, st);
+        return direct ? launch_tiles<T, TO, kMode, 64, 64, 2, 2, true, 4, 4>(g, st)
+                      : launch_tiles<T, TO, kMode, 64, 64, 2, 2, false, 2, 2>(g, st);
       } else {
         return fail(HPSPMM_ERR_INVALID_ARG, "no product of these types");
       }

@@ -58,16 +58,17 @@ struct Mfma<float> {
 typedef __attribute__((address_space(3))) char lds_char;
 typedef short short4_t __attribute__((ext_vector_type(4)));
 
+constexpr int kStepChunks = 8;  // 16-byte chunks of the contraction a step: whole lines of a row operand
+
 // One operand of one output tile.
-// kC: 16-byte chunks of the contraction a step (4 or 8).
-template <class T, bool kCol, int kB, int kThreads, bool kDirect, int kC>
+template <class T, bool kCol, int kB, int kThreads, bool kDirect>
 struct Operand {
   static constexpr int kSize = (int)sizeof(T);
   static constexpr int kChunk = 16 / kSize;    // elements of a 16-byte chunk
-  static constexpr int kDepth = kC * kChunk;   // terms of the contraction a step
-  static constexpr int kBytes = kB * kC * 16;  // of LDS a step
-  static constexpr int kPer = kB * kC / kThreads;  // chunks a thread brings in a step
-  static constexpr int kRowChunks = kCol ? kB / kChunk : kC;  // chunks of a row in LDS
+  static constexpr int kDepth = kStepChunks * kChunk;  // terms of the contraction a step
+  static constexpr int kBytes = kB * kStepChunks * 16;  // of LDS a step
+  static constexpr int kPer = kB * kStepChunks / kThreads;  // chunks a thread brings in a step
+  static constexpr int kRowChunks = kCol ? kB / kChunk : kStepChunks;  // chunks of a row in LDS
   static constexpr uint32_t kNowhere = 0xFFFFFFF0u;  // an offset beyond the buffer: the load gives zeros
   using Chunk = typename Pack<T, kChunk, true>::type;
 
@@ -78,7 +79,7 @@ struct Operand {
   uint32_t offset[kDirect ? kPer : 1];
 
   static __device__ __forceinline__ int swizzle(int r) {
-    if constexpr (!kCol) return kC == 8 ? r & 7 : (r >> 2) & 3;
+    if constexpr (!kCol) return r & 7;
     else if constexpr (kSize == 2) return (((r & 3) | ((r >> 1) & 4)) << 1) & (kRowChunks - 1);
     else return (((r >> 2) & 3) << 2) & (kRowChunks - 1);
   }
@@ -175,7 +176,7 @@ struct Operand {
     const int lane = threadIdx.x & 63, low = lane & 15, high = lane >> 4;
     if constexpr (!kCol) {
       const int r = at + low;
-      return *reinterpret_cast<const Frag*>(lds + r * (kC * 16) + (((h * 4 + high) ^ swizzle(r)) << 4));
+      return *reinterpret_cast<const Frag*>(lds + r * (kStepChunks * 16) + (((h * 4 + high) ^ swizzle(r)) << 4));
     } else if constexpr (kSize == 2) {
       Frag f;
 #pragma unroll
@@ -224,11 +225,11 @@ __device__ __forceinline__ int64_t xcd_tile(int64_t tiles) {
   return b / kXcds < per && t < tiles ? t : -1;
 }
 
-template <class T, class TO, int kMode, int kBM, int kBN, int kWM, int kWN, bool kDirect, int kC, int kStagesA, int kStagesB, bool kSplit = false>
+template <class T, class TO, int kMode, int kBM, int kBN, int kWM, int kWN, bool kDirect, int kStagesA, int kStagesB, bool kSplit = false>
 __global__ __launch_bounds__(64 * kWM * kWN, 2) void grouped_tile_kernel(GroupedArgs g, int col_tiles) {
   constexpr int kThreads = 64 * kWM * kWN;
-  using OpA = Operand<T, kMode == kGradW, kBM, kThreads, kDirect, kC>;
-  using OpB = Operand<T, kMode != kForward, kBN, kThreads, kDirect, kC>;
+  using OpA = Operand<T, kMode == kGradW, kBM, kThreads, kDirect>;
+  using OpB = Operand<T, kMode != kForward, kBN, kThreads, kDirect>;
   using Frag = typename Mfma<T>::frag;
   constexpr int FM = kBM / kWM / 16, FN = kBN / kWN / 16, kDepth = OpA::kDepth;
   constexpr int kLdsA = kStagesA * OpA::kBytes, kLds = kLdsA + kStagesB * OpB::kBytes;
@@ -288,7 +289,7 @@ __global__ __launch_bounds__(64 * kWM * kWN, 2) void grouped_tile_kernel(Grouped
   float4_t acc[FM][FN] = {};
   // The products of one step, sum by sum of 16 rows; `between(i)` after the i-th.  The next half of the step is read
   // while this one is multiplied.
-  constexpr int H = kC / 4;
+  constexpr int H = kStepChunks / 4;
   auto multiply = [&](const char* lds_a, const char* lds_b, auto between) {
     Frag fa[H][FM], fb[H][FN];
 #pragma unroll

@@ -220,7 +220,6 @@ HPSPMM_API int hpspmm_rows_plan_create(int64_t max_rows, int64_t max_ids, int64_
     delete p;
     return fail(HPSPMM_ERR_ALLOC, "device allocation of %lld bytes for the plan failed", (long long)bytes);
   }
-  p->workspace_bytes = bytes;
   char* at = p->arena;
   auto take = [&](int64_t w) {
     char* q = at;

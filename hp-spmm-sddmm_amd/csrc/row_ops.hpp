@@ -9,7 +9,6 @@ struct hpspmm_rows_plan {
   int device = 0;
   int64_t max_rows = 0, max_ids = 0, max_width = 0;
   char* arena = nullptr;
-  int64_t workspace_bytes = 0;
   uint32_t* d_keys[2] = {nullptr, nullptr};  // [max_rows] ids, sorted
   int32_t* d_vals[2] = {nullptr, nullptr};   // [max_rows] the rows they belong to
   uint32_t* d_hist = nullptr;                // [tiles * bins] counts per digit and tile of rows
