@@ -263,7 +263,7 @@ namespace hpspmm_host {
 
 // ---- plan_util.hip -------------------------------------------------------------------------
 
-// Whether workgroup b of a launch runs on XCD b % 8 on the current device (probed once per device
+// Whether workgroups are dealt to the 8 XCDs in turn on the current device (probed once per device
 // and process; `assume` = 0 / 1 skips the probe).
 bool xcd_dealing_holds(hipStream_t st, int assume);
 

@@ -51,10 +51,13 @@ int check_dims(int64_t rows, int64_t cols, int64_t nnz, int64_t k) {
 }
 
 // The routed strategy pins column slices to XCDs and xcd_remap deals row ranges to them; both rely on
-// workgroup b of a launch running on XCD b % 8.  That holds for the whole device (8 XCDs, 256 CUs);
-// a partitioned device (fewer XCDs behind one HIP device) or a future dispatcher would break it
+// the workgroups of a launch being dealt to the XCDs in turn: b, b + 8, b + 16 ... run on one XCD, eight
+// neighbours on eight of them.  Which XCD a launch begins with belongs to its hardware queue (of the
+// first streams of a process 0, 5, 6 and 7 were seen, the same in every launch of a stream) and does not
+// matter: no strategy asks for a particular one.  The dealing holds for the whole device (8 XCDs, 256
+// CUs); a partitioned device (fewer XCDs behind one HIP device) or a future dispatcher would break it
 // silently, so it is measured once per device: 512 probe workgroups report the XCD they ran on.
-// 0 = not probed yet, 1 = workgroup b runs on XCD b % 8, 2 = it does not (the plan then keeps to the
+// 0 = not probed yet, 1 = they are dealt in turn, 2 = they are not (the plan then keeps to the
 // strategies that do not depend on it).
 namespace {
 constexpr int kMaxDevices = 64;
@@ -86,7 +89,7 @@ bool xcd_dealing_holds(hipStream_t st, int assume) {
     return false;  // not cached: a transient failure should not decide for the life of the process
   }
   int match = 0;
-  for (int b = 0; b < kProbeBlocks; ++b) match += ids[b] == b % hpspmm::kXcds;
+  for (int b = 0; b < kProbeBlocks; ++b) match += ids[b] == (ids[0] + b) % hpspmm::kXcds;
   g_xcd_state[dev] = match == kProbeBlocks ? 1 : 2;
   return g_xcd_state[dev] == 1;
 }

@@ -9,10 +9,11 @@
 //   * every column belongs to one of 8 slices: the most referenced columns by
 //     popularity rank, round robin, so that the slices carry equal load, the
 //     rest by a hash of the index.  Slice x of B is only ever read by
-//     workgroups running on XCD x (workgroup b runs on XCD b % 8), so each L2
-//     sees an eighth of the columns and keeps the hot ones (measured on the
-//     233k-vertex social graph, K=128: 6.6 ms -> 4.5 ms).  A slice can further
-//     be cut into up to 7 phases that an XCD works through one after the other,
+//     workgroups running on XCD x (workgroup b runs on XCD b % 8, counted
+//     from the XCD that its launch begins with), so each L2 sees an eighth
+//     of the columns and keeps the hot ones (measured on the 233k-vertex
+//     social graph, K=128: 6.6 ms -> 4.5 ms).  A slice can further be cut
+//     into up to 7 phases that an XCD works through one after the other,
 //     each with the same mix of hot and cold columns;
 //   * the most referenced rows of B are additionally copied, slice by slice,
 //     into a compact buffer at the start of every SpMM, which takes them off

@@ -167,7 +167,7 @@ __device__ __forceinline__ float4 load_b_hub_ld(const float* __restrict__ B, con
 }
 
 // Workgroups are dealt to the XCDs round-robin (workgroup b runs on XCD
-// b % 8).  Remapping so that XCD x receives the x-th contiguous eighth of the
+// b % 8, counted from the one that the launch begins with).  Remapping so that XCD x receives the x-th contiguous eighth of the
 // logical workgroups keeps neighbouring rows (similar column sets) behind one
 // L2.  Returns -1 for the padding workgroups of the rounded-up grid.
 __device__ __forceinline__ int64_t xcd_remap(int64_t b, int64_t nblocks, bool remap) {

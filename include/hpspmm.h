@@ -126,7 +126,7 @@ typedef struct hpspmm_plan_options {
   int32_t routed_lds_rows;    /* column tiles of the routed strategy: rows of B a workgroup keeps in LDS (at most
                                  what fits; -1 = none) */
   int32_t xcd_dealing;        /* 0: probe how workgroups are dealt to the XCDs (once per device and process);
-                                 1: take workgroup b to run on XCD b % 8; 2: take it not to */
+                                 1: take workgroups to be dealt to the 8 XCDs in turn; 2: take them not to */
   int32_t no_column_tiles;    /* 1: a k outside 32 / 64 / 128 never gets the sweep / routed / ordered
                                  layouts in column tiles */
   int32_t row_tiles_min_k;    /* row tiles serve a k outside the tuned set only from this k up */
@@ -168,7 +168,7 @@ int hpspmm_version(void);
 
 /*
  * What the library sees of the current device (hipDeviceProp figures, and whether
- * the probe of hpspmm_plan_create found workgroup b on XCD b % 8).  For reports:
+ * the probe of hpspmm_plan_create found workgroups dealt to the XCDs in turn).  For reports:
  * the benchmark prices the L2 -> CU path with the clock given here.  No
  * counterpart in the reference.
  */
@@ -180,7 +180,7 @@ typedef struct hpspmm_device_info {
   int64_t l2_bytes;          /* as hipDeviceProp reports it (one XCD's) */
   int64_t lds_bytes_per_cu;
   int64_t global_bytes;
-  int32_t xcd_dealing;       /* 1: workgroup b of a launch runs on XCD b % 8 */
+  int32_t xcd_dealing;       /* 1: workgroups b, b + 8, b + 16 ... of a launch run on one XCD, 8 neighbours on 8 */
   char arch[60];
 } hpspmm_device_info;
 int hpspmm_get_device_info(hpspmm_device_info *info_out);
@@ -238,10 +238,12 @@ const char *hpspmm_last_error(void);
  * on computing the old matrix.
  * The strategies that place work on particular XCDs (routed; the row-range
  * dealing of the others) are used only if a probe launch, once per device and
- * process, has seen workgroup b run on XCD b % 8, which is how the whole
- * (unpartitioned) device deals them; otherwise the plan keeps to segments,
- * rows and ordered without that placement (hpspmm_plan_options.xcd_dealing
- * replaces the probe by the caller's word).
+ * process, has seen workgroups dealt to the 8 XCDs in turn, which is how the
+ * whole (unpartitioned) device deals them - from whichever XCD the stream's
+ * hardware queue begins with, so it does not matter on which stream the first
+ * plan is made; otherwise the plan keeps to segments, rows and ordered without
+ * that placement (hpspmm_plan_options.xcd_dealing replaces the probe by the
+ * caller's word).
  */
 int hpspmm_plan_create(int64_t rows, int64_t cols, int64_t nnz, const int32_t *d_rowptr,
                        const int32_t *d_col, int64_t k, uint32_t flags, void *stream,

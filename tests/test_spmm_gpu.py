@@ -1272,3 +1272,47 @@ def test_column_tiles(pkg, oracle, gpu, k, tile, ntiles):
     # small and unforced: no tiles, the plan for any multiple of 4
     _, info = _run(pkg, gpu, g, B, capi.PLAN_DEFAULT)
     assert info["strategy"] in (capi.STRATEGY_ROWS, capi.STRATEGY_SEGMENTS) and info["k"] == k and info["column_tiles"] == 1, info
+
+
+_FIRST_PLAN_ON_A_STREAM = """
+import importlib, sys
+import numpy as np
+import torch
+sys.path.insert(0, sys.argv[1])
+pkg = importlib.import_module("hp-spmm-sddmm_amd")
+from oracle import oracle
+capi, graphs = pkg.capi, pkg.graphs
+dev = torch.device("cuda:0")
+streams = [torch.cuda.Stream() for _ in range(3)]
+for s in streams:
+    with torch.cuda.stream(s):
+        torch.ones(100, device=dev).mul_(2)
+torch.cuda.synchronize()
+g = graphs.make_graph("c2_social", 0.1)
+B = graphs.make_dense("c2_social", g.cols, 128)
+d = [torch.from_numpy(a).to(dev) for a in (g.rowptr, g.col, g.val, B)]
+C = torch.full((g.rows, 128), float("nan"), device=dev)
+torch.cuda.synchronize()
+plan = capi.Plan(g.rows, g.cols, d[0], d[1], 128, capi.PLAN_NO_SWEEP, stream=streams[int(sys.argv[2])])
+capi.csr_spmm(plan, *d, C, stream=streams[int(sys.argv[2])])
+torch.cuda.synchronize()
+C64, S64 = oracle.csr_spmm_f64(g.rowptr, g.col, g.val, B)
+err, pos = oracle.max_norm_err(C.cpu().numpy(), C64, S64)
+print("RESULT", plan.info["strategy"], capi.device_info()["xcd_dealing"], err)
+"""
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_xcd_placement_is_seen_from_any_stream(pkg, gpu, which):
+    """A process whose first plan is made on a stream of its own, after others were used: workgroups are dealt to the
+    XCDs in turn from whichever XCD that stream's queue begins with, and the plan is the one that it would be anyway."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", _FIRST_PLAN_ON_A_STREAM, root, str(which)], capture_output=True, text=True,
+                       timeout=100)
+    assert r.returncode == 0, r.stdout + r.stderr
+    line = [q for q in r.stdout.splitlines() if q.startswith("RESULT")][-1].split()
+    assert int(line[1]) == pkg.capi.STRATEGY_ROUTED and int(line[2]) == 1, line
+    assert float(line[3]) <= TOL, line

@@ -4,9 +4,6 @@ Tolerances follow from the arithmetic that the operators promise (sums in 32 bit
 u = eps / 2 of a type: a product or sum of L terms formed in 32 bits is off by at most (L + 2) * 2 * u32 * sum |terms|
 (2: a matrix instruction may cut where an addition rounds), its rounding to the output's type by u * |value|, or by half
 of that type's smallest step where values are below its normal range.
-
-The file's name puts it behind the tests of the sparse products: their plans look once per process at how workgroups are
-dealt to the XCDs, and a process that has used streams of its own before, as two tests here do, deals them otherwise.
 """
 import numpy as np
 import pytest
