@@ -93,6 +93,7 @@ EXPORTS = (
     "hpspmm_static_workspace_init", "hpspmm_csr_spmm_timed_min", "hpspmm_get_device_info",
     "hpspmm_rows_plan_create", "hpspmm_rows_plan_destroy", "hpspmm_embedding_lookup", "hpspmm_embedding_grad",
     "hpspmm_group_rows", "hpspmm_grouped_mm", "hpspmm_grouped_mm_grad_x", "hpspmm_grouped_mm_grad_w",
+    "hpspmm_grouped_tiling",
 )
 
 _i64 = ctypes.c_int64
@@ -190,6 +191,7 @@ def lib():
         L.hpspmm_grouped_mm.argtypes = [_i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _i64, _p, _p, _i64, i, _p]
         L.hpspmm_grouped_mm_grad_x.argtypes = L.hpspmm_grouped_mm.argtypes
         L.hpspmm_grouped_mm_grad_w.argtypes = [_p, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _i64, i, i, i, _p]
+        L.hpspmm_grouped_tiling.argtypes = [i, _i64, _i64, _i64, _i64, i, i, ctypes.POINTER(i), ctypes.POINTER(i)]
         _lib = L
     return _lib
 
@@ -580,3 +582,14 @@ def grouped_mm_grad_w(plan, dy, x, offsets, dw, accumulate=False, stream=None):
              ld_x, _offsets(offsets, "offsets", groups + 1, device), dw_p, ld_dw, stride_dw, kind, dw_kind,
              bool(accumulate))
     return dw
+
+
+PRODUCTS = ("grouped_mm", "grouped_mm_grad_x", "grouped_mm_grad_w")
+
+
+def grouped_tiling(product, rows, groups, k, m, kind, whole16=True):
+    """(edge of the output tiles, parts of the rows) of one of PRODUCTS, through hpspmm_grouped_tiling; kind: F32, BF16, F16."""
+    edge, parts = ctypes.c_int(), ctypes.c_int()
+    check(lib().hpspmm_grouped_tiling(PRODUCTS.index(product), rows, groups, k, m, kind, bool(whole16), ctypes.byref(edge),
+                                      ctypes.byref(parts)))
+    return edge.value, parts.value

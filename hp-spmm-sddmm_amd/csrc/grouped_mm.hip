@@ -93,6 +93,18 @@ int row_splits(const hpspmm::GroupedArgs& g, int64_t depth) {
   return (int)std::max<int64_t>(1, std::min(hpspmm::kSplitTiles / std::max<int64_t>(tiles, 1), steps / 4));
 }
 
+// How a product is cut: the edge of its output tiles, and the parts of the rows (1 = none) for the gradient of the weights.
+struct Tiling {
+  int edge, splits;
+};
+Tiling tiling_of(int mode, const hpspmm::GroupedArgs& g, int64_t size, bool direct) {
+  if (mode == hpspmm::kGradW) {
+    const int splits = row_splits(g, 128 / size);
+    if (splits > 1) return {hpspmm::kSplitEdge, splits};
+  }
+  return {tile_edge(mode, g, size == 4, size == 2 && direct), 1};
+}
+
 // The gradient of the weights in parts: sums in 32 bits of every part and tile to the plan's workspace, then their sum.
 template <class T, class TO>
 int launch_split(hpspmm::GroupedArgs g, int splits, bool direct, hipStream_t st) {
@@ -122,11 +134,10 @@ int launch_grouped(const hpspmm::GroupedArgs& g, int dtype, int out_type, hipStr
     return dispatch_dtype(out_type, [&](auto o) {
       using TO = decltype(o);
       if constexpr (std::is_same_v<T, TO> || (kMode == hpspmm::kGradW && std::is_same_v<TO, float>)) {
+        const auto [edge, splits] = tiling_of(kMode, g, size, direct);
         if constexpr (kMode == hpspmm::kGradW) {
-          const int splits = row_splits(g, 128 / (int64_t)sizeof(T));
           if (splits > 1) return launch_split<T, TO>(g, splits, direct, st);
         }
-        const int edge = tile_edge(kMode, g, sizeof(T) == 4, sizeof(T) == 2 && direct);
         if constexpr (sizeof(T) == 2) {
           if (edge == 256) return launch_tiles<T, TO, kMode, 256, 256, 2, 4, true, 3, 2>(g, st);
         }
@@ -146,6 +157,22 @@ int launch_grouped(const hpspmm::GroupedArgs& g, int dtype, int out_type, hipStr
 }
 
 }  // namespace
+
+HPSPMM_API int hpspmm_grouped_tiling(int product, int64_t rows, int64_t groups, int64_t k, int64_t m, int dtype, int whole16,
+                                     int* edge_out, int* parts_out) {
+  if (!edge_out || !parts_out) return fail(HPSPMM_ERR_INVALID_ARG, "edge_out or parts_out is NULL");
+  *edge_out = *parts_out = 0;
+  if (product < hpspmm::kForward || product > hpspmm::kGradW) return fail(HPSPMM_ERR_INVALID_ARG, "unknown product %d", product);
+  static const int32_t none = 0;
+  if (int rc = check_grouped(rows, groups, k, m, &none, dtype)) return rc;
+  if (groups == 0 || (product != hpspmm::kGradW && rows == 0)) return HPSPMM_OK;
+  hpspmm::GroupedArgs g{};
+  g.rows = rows, g.groups = groups, g.k = (int32_t)k, g.m = (int32_t)m;
+  const auto [edge, splits] = tiling_of(product, g, dtype_size(dtype), whole16 != 0);
+  *edge_out = edge;
+  *parts_out = splits;
+  return HPSPMM_OK;
+}
 
 HPSPMM_API int hpspmm_grouped_mm(int64_t rows, int64_t groups, int64_t k, int64_t m, const void* d_x, int64_t ld_x,
                                  const void* d_w, int64_t ld_w, int64_t stride_w, const int32_t* d_offsets, void* d_y,

@@ -509,6 +509,17 @@ int hpspmm_grouped_mm_grad_w(hpspmm_rows_plan *plan, int64_t rows, int64_t group
                              void *d_dw, int64_t ld_dw, int64_t stride_dw, int dtype, int dw_type, int accumulate,
                              void *stream);
 
+/*
+ * How one of these products would be cut, for reports and tests (no device is
+ * touched): product 0 / 1 / 2 = hpspmm_grouped_mm / _grad_x / _grad_w; whole16:
+ * the rows of both operands are whole 16-byte pieces at multiples of 16 bytes.
+ * edge = edge of the output tiles; parts = parts that the rows of every group
+ * are cut into, whose sums are joined by a second launch (1: not cut); both 0
+ * where nothing would be launched.
+ */
+int hpspmm_grouped_tiling(int product, int64_t rows, int64_t groups, int64_t k, int64_t m, int dtype, int whole16,
+                          int *edge_out, int *parts_out);
+
 #ifdef __cplusplus
 }
 #endif

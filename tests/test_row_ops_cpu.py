@@ -115,3 +115,45 @@ def test_python_entry_points_refuse_host_tensors(pkg):
         capi.grouped_mm(table, torch.zeros(2, 3, 16), torch.zeros(3, dtype=torch.int32), torch.zeros(8, 3))
     with pytest.raises(TypeError, match="GPU memory"):
         capi.grouped_mm_grad_x(torch.zeros(8, 3), torch.zeros(2, 3, 16), torch.zeros(3, dtype=torch.int32), table)
+
+
+# Sizes (rows, groups, k, m) of grouped products that between them are cut in every way there is; the GPU tests run them.
+TILED = [(300, 5, 129, 65), (1000, 7, 256, 384), (700, 16, 1032, 1032), (9000, 5, 264, 4104), (9000, 5, 4104, 264),
+         (9000, 5, 1028, 2052), (9000, 5, 1001, 1003), (2000, 16, 1016, 1000), (2000, 16, 1001, 1003), (12000, 3, 520, 1032),
+         (9000, 2, 200, 89)]
+
+
+def tilings(capi, kind, size, case):
+    """{(product, whole rows, edge, in parts)} of one case; rows are whole where both lengths are multiples of 16 bytes."""
+    rows, groups, k, m = case
+    whole = k * size % 16 == 0 and m * size % 16 == 0
+    cut = {q: capi.grouped_tiling(q, rows, groups, k, m, kind, whole) for q in capi.PRODUCTS}
+    return {(q, whole, edge, parts > 1) for q, (edge, parts) in cut.items()}
+
+
+@pytest.mark.parametrize("kind, size", [(0, 4), (1, 2), (2, 2)])
+def test_the_tested_products_are_cut_in_every_way(pkg, kind, size):
+    """Every tile kernel that a call can reach is reached by a size in TILED (a rule that is changed must not leave a
+    kernel behind untested)."""
+    capi = pkg.capi
+    reached = set().union(*(tilings(capi, kind, size, case) for case in TILED))
+    edges = {True: (256, 128, 64) if size == 2 else (128, 64), False: (128, 64)}
+    every = {(q, whole, edge, False) for q in capi.PRODUCTS for whole in edges for edge in edges[whole]}
+    every |= {("grouped_mm_grad_w", whole, 128, True) for whole in edges}
+    assert reached == every, (sorted(every - reached), sorted(reached - every))
+
+
+def test_tiling_refuses(pkg):
+    capi = pkg.capi
+    edge, parts = ctypes.c_int(), ctypes.c_int()
+    call = lambda *a, e=ctypes.byref(edge), p=ctypes.byref(parts): capi.lib().hpspmm_grouped_tiling(*a, e, p)  # noqa: E731
+    assert call(0, 8, 2, 16, 32, 1, 1) == capi.OK and edge.value and parts.value == 1
+    for bad in ((3, 8, 2, 16, 32, 1, 1), (-1, 8, 2, 16, 32, 1, 1), (0, -1, 2, 16, 32, 1, 1), (0, 8, -1, 16, 32, 1, 1),
+                (0, 8, 2, 0, 32, 1, 1), (0, 8, 2, 16, 0, 1, 1), (0, 8, 2, 16, 32, 3, 1)):
+        assert call(*bad) == capi.ERR_INVALID_ARG and (edge.value, parts.value) == (0, 0)
+    assert call(0, 8, 2, 16, 32, 1, 1, e=None) == capi.ERR_INVALID_ARG
+    assert call(0, 8, 2, 16, 32, 1, 1, p=None) == capi.ERR_INVALID_ARG
+    # nothing is launched for no groups, and for no rows but to clear the gradient of the weights
+    assert capi.grouped_tiling("grouped_mm", 0, 2, 16, 32, capi.BF16) == (0, 0)
+    assert capi.grouped_tiling("grouped_mm_grad_w", 8, 0, 16, 32, capi.BF16) == (0, 0)
+    assert capi.grouped_tiling("grouped_mm_grad_w", 0, 2, 16, 32, capi.BF16) == (64, 1)

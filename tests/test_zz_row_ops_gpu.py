@@ -8,6 +8,8 @@ of that type's smallest step where values are below its normal range.
 import numpy as np
 import pytest
 
+from test_row_ops_cpu import TILED
+
 pytestmark = pytest.mark.gpu
 
 KINDS = ["float32", "bfloat16", "float16"]
@@ -682,3 +684,18 @@ def test_operands_that_do_not_fit_are_refused(pkg, gpu):
         with pytest.raises(error):
             call()
             pytest.fail(f"call {n} was not refused")
+
+
+# ---- paths that the sizes above do not reach ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("layout", ["contiguous", "aligned_slice", "odd_slice"])
+@pytest.mark.parametrize("rows, groups, k, m", TILED)
+def test_grouped_products_cut_in_every_way(pkg, gpu, kind, layout, rows, groups, k, m):
+    """Every edge of the output tiles, whole rows and any others, with parts of tiles at both ends."""
+    test_grouped_products(pkg, gpu, kind, layout, "ragged", rows, groups, k, m)
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float16"])
+def test_gradient_of_weights_added_in_their_type_in_the_largest_tiles(pkg, gpu, kind):
+    test_gradient_of_weights_added_in_their_type(pkg, gpu, kind, "contiguous", 2000, 16, 1016, 1000)
