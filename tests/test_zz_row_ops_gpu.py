@@ -699,3 +699,36 @@ def test_grouped_products_cut_in_every_way(pkg, gpu, kind, layout, rows, groups,
 @pytest.mark.parametrize("kind", ["bfloat16", "float16"])
 def test_gradient_of_weights_added_in_their_type_in_the_largest_tiles(pkg, gpu, kind):
     test_gradient_of_weights_added_in_their_type(pkg, gpu, kind, "contiguous", 2000, 16, 1016, 1000)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("id_kind", ["int32", "int64"])
+@pytest.mark.parametrize("short, columns", [(0, 1024), (4, 1024), (60, 2112), (64, 2112)])
+def test_lookup_of_large_outputs(pkg, gpu, kind, id_kind, short, columns):
+    """More than 64 MB of rows at multiples of 128 bytes (written past the caches), `short` columns shorter than their
+    places in memory (as many bytes in 32 bits; a last piece of 16 bytes that is not whole stays so), in one and two tiles
+    of columns, and a number of rows that leaves the last workgroup short."""
+    torch = _torch()
+    if kind == "float32":
+        columns, short = columns // 2, short // 2 + (short % 8 == 4)
+    g = _gen(gpu, columns + short)
+    width, vocab = columns - short, 3001
+    n = -(-(70 << 20) // (width * torch.finfo(_t(kind)).bits // 8)) | 1
+    table = torch.full((vocab, columns), float("nan"), device=gpu, dtype=_t(kind))[:, :width]
+    table.copy_(torch.randn(vocab, width, device=gpu, generator=g))
+    ids = _ids(gpu, g, n, vocab, id_kind)
+    big = torch.full((n + 2, columns), 77.0, device=gpu, dtype=_t(kind))
+    out = big[1:n + 1, :width]
+    out.fill_(float("nan"))
+    scale = 5.65685424949
+    pkg.capi.embedding_lookup(table, ids, out, scale=scale)
+    here = _in_table(ids, vocab)
+    f = torch.finfo(out.dtype)
+    for r in range(0, n, 8192):  # (64-bit copies of the whole would be large)
+        rows = slice(r, min(r + 8192, n))
+        want = table[torch.where(here[rows], ids[rows].long(), 0)].double() * float(np.float32(scale))
+        want[~here[rows]] = 0.0
+        tol = want.abs() * (f.eps / 2 + 2.0 ** -24) * (1 + 2.0 ** -8) + f.smallest_normal * f.eps / 2
+        assert bool(((out[rows].double() - want).abs() <= tol).all()), r
+    assert not out[~here].any()
+    assert bool((big[0] == 77.0).all() and (big[-1] == 77.0).all() and (big[:, width:] == 77.0).all())
