@@ -732,3 +732,61 @@ def test_lookup_of_large_outputs(pkg, gpu, kind, id_kind, short, columns):
         assert bool(((out[rows].double() - want).abs() <= tol).all()), r
     assert not out[~here].any()
     assert bool((big[0] == 77.0).all() and (big[-1] == 77.0).all() and (big[:, width:] == 77.0).all())
+
+
+@pytest.mark.parametrize("id_kind", ["int32", "int64"])
+@pytest.mark.parametrize("how", ["mixed", "one", "none"])
+@pytest.mark.parametrize("n, groups", [(20000, (1 << 20) + 5), (1100000, 300), (1100000, (1 << 20) + 5)])
+def test_group_rows_of_three_digits_and_many_tiles(pkg, gpu, id_kind, how, n, groups):
+    test_group_rows(pkg, gpu, id_kind, how, n, groups)
+
+
+@pytest.mark.parametrize("kind, out_kind", [("bfloat16", "same"), ("float16", "float32"), ("float32", "bfloat16")])
+@pytest.mark.parametrize("layout", ["contiguous", "odd_slice"])
+@pytest.mark.parametrize("how", ["mixed", "none"])
+@pytest.mark.parametrize("n, vocab, width", [(20000, (1 << 20) + 5, 8), (1100000, (1 << 20) + 5, 5)])
+def test_lookup_gradient_behind_the_longer_sorts(pkg, gpu, kind, out_kind, layout, how, n, vocab, width):
+    test_lookup_gradient(pkg, gpu, kind, out_kind, layout, how, n, vocab, width)
+
+
+@pytest.mark.parametrize("kind, out_kind", [("bfloat16", "bfloat16"), ("float16", "float32"), ("float32", "bfloat16")])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_lookup_gradient_of_many_rows_over_few_ids(pkg, gpu, kind, out_kind, accumulate):
+    """One digit, more tiles of rows than a workgroup adds up by itself (the sums of the reference on the host: 64-bit
+    atomic additions to few rows crawl)."""
+    torch = _torch()
+    g = _gen(gpu, 14)
+    n, vocab, width = 1100000, 300, 9
+    ids = torch.randint(-30, vocab + 30, (n,), device=gpu, generator=g)
+    grad = torch.randn(n, width, device=gpu, generator=g).to(_t(kind))
+    start = torch.randn(vocab, width, device=gpu, generator=g).to(_t(out_kind))
+    out = pkg.capi.embedding_grad(pkg.capi.RowsPlan(n, vocab, width), ids, grad, start.clone(), scale=0.75, accumulate=accumulate)
+    value, absolute, count = _grad_reference(ids.cpu(), grad.cpu(), vocab, 0.75)
+    if accumulate:
+        value, absolute = value + start.cpu().double(), absolute + start.cpu().double().abs()
+    _check(out.cpu(), value, absolute, count + accumulate)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("out_kind", KINDS)
+@pytest.mark.parametrize("layout", ["contiguous", "aligned_slice", "odd_slice"])
+@pytest.mark.parametrize("n, vocab, width", [(1, 1, 1), (100, 1000, 64), (3001, 257, 129), (9000, 40, 520), (2000, 90, 12)])
+def test_lookup_gradient_of_any_pair_of_types(pkg, gpu, kind, out_kind, layout, n, vocab, width):
+    test_lookup_gradient(pkg, gpu, kind, out_kind, layout, "mixed", n, vocab, width)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n, vocab, width", [(20, 7, 24), (900, 40, 129), (9000, 300, 64), (40000, 3, 16)])
+def test_lookup_gradient_of_padding_that_is_nan(pkg, gpu, kind, n, vocab, width):
+    """What stands in the rows of ids outside the table reaches nothing: the same bits as with zeros there."""
+    torch = _torch()
+    g = _gen(gpu, n)
+    ids = _ids(gpu, g, n, vocab, "int64")
+    grad = torch.randn(n, width, device=gpu, generator=g).to(_t(kind))
+    out = _in_table(ids, vocab).logical_not()
+    plan = pkg.capi.RowsPlan(n, vocab, width)
+    got = []
+    for fill in (0.0, float("nan"), float("inf")):
+        grad[out] = fill
+        got.append(pkg.capi.embedding_grad(plan, ids, grad, torch.full((vocab, width), 3.0, device=gpu)))
+    assert not torch_isnan(got[0]) and torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
