@@ -790,3 +790,20 @@ def test_lookup_gradient_of_padding_that_is_nan(pkg, gpu, kind, n, vocab, width)
         grad[out] = fill
         got.append(pkg.capi.embedding_grad(plan, ids, grad, torch.full((vocab, width), 3.0, device=gpu)))
     assert not torch_isnan(got[0]) and torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+
+
+def test_a_call_on_a_stream_that_is_not_the_current_one(pkg, gpu):
+    """... runs behind what that stream has under way: the inputs are written there, by work that takes a while."""
+    torch = _torch()
+    s = _routed_state(pkg, gpu, "bfloat16", n=2000, seed=41)
+    want = pkg.capi.embedding_lookup(s["table"], s["tokens"], torch.empty_like(s["h"]), scale=2.0)
+    table, s["table"] = s["table"], torch.zeros_like(s["table"])
+    side, busy = torch.cuda.Stream(), torch.randn(4096, 4096, device=gpu)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(8):
+            busy = (busy @ busy).clamp_(-1, 1)
+        s["table"].copy_(table)
+    pkg.capi.embedding_lookup(s["table"], s["tokens"], s["h"], scale=2.0, stream=side)
+    side.synchronize()
+    assert torch.equal(s["h"], want)
