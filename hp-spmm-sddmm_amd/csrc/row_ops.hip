@@ -166,6 +166,8 @@ struct SumShape {
   int64_t col_tiles, chunks, pitch;
 };
 constexpr int kMinChunkLog2 = 2, kMaxChunkLog2 = 7;
+// (a launch holds fewer than 2^32 threads: 2^24 - 1 workgroups, some of which fill rows with zeros beside the sums)
+constexpr int64_t kMostChunks = ((int64_t)1 << 24) - ((int64_t)1 << 21);
 SumShape sum_shape(int64_t n, int64_t width, int64_t per16) {
   SumShape s{};
   const int64_t vecs = ceil_div(width, per16);
@@ -174,6 +176,7 @@ SumShape sum_shape(int64_t n, int64_t width, int64_t per16) {
   // chunks as long as leaves 1024 of them a column tile, at most 128 rows
   s.chunk_log2 = kMinChunkLog2;
   while (s.chunk_log2 < kMaxChunkLog2 && (n * s.col_tiles) >> (s.chunk_log2 + 1) >= 1024) ++s.chunk_log2;
+  while (ceil_div(n, (int64_t)1 << s.chunk_log2) > kMostChunks) ++s.chunk_log2;
   if (n <= 32) s.chunk_log2 = 5;  // one chunk: no sum crosses it, one launch less
   s.chunks = ceil_div(n, (int64_t)1 << s.chunk_log2);
   s.pitch = ceil_div(width, 8) * 8;

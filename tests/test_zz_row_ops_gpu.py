@@ -792,6 +792,30 @@ def test_lookup_gradient_of_padding_that_is_nan(pkg, gpu, kind, n, vocab, width)
     assert not torch_isnan(got[0]) and torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
 
 
+def test_lookup_gradient_of_as_many_rows_as_there_may_be(pkg, gpu):
+    """2^31 - 2 rows (chunks of 128 of them are as many as a launch has no room for): whole numbers, so every sum is exact."""
+    torch = _torch()
+    n = (1 << 31) - 2
+    if torch.cuda.mem_get_info()[0] < 120 << 30:
+        pytest.skip("needs 120 GB of GPU memory")
+    ids = torch.zeros(n, dtype=torch.int32, device=gpu)
+    ids[n // 2:] = 1
+    ids[5::1 << 20] = -1
+    grad = torch.zeros(n, 1, dtype=torch.float16, device=gpu)
+    for at in (0, 5, 127, 128, n // 2 - 1, n // 2, n // 2 + 12345, n - 129, n - 2, n - 1):
+        grad[at] = at % 7 + 1
+    want = torch.zeros(3, device=gpu)
+    at = torch.nonzero(grad[:, 0]).flatten()
+    at = at[ids[at] >= 0]
+    want.index_add_(0, ids[at].long(), grad[at, 0].float())
+    plan = pkg.capi.RowsPlan(n, 3, 1)
+    for accumulate in (False, True):
+        out = torch.full((3, 1), 64.0 if accumulate else float("nan"), device=gpu)
+        pkg.capi.embedding_grad(plan, ids, grad, out, accumulate=accumulate)
+        assert torch.equal(out[:, 0], want + 64.0 if accumulate else want), accumulate
+    plan.destroy()
+
+
 def test_a_call_on_a_stream_that_is_not_the_current_one(pkg, gpu):
     """... runs behind what that stream has under way: the inputs are written there, by work that takes a while."""
     torch = _torch()
