@@ -470,6 +470,8 @@ def _offsets(t, name, entries, device):
 def _call_on(device, stream, function, *args):
     """function(*args, stream) with `device` current, on `stream` or that device's current one."""
     t, index = _with_torch(), device.index
+    if stream is not None and getattr(stream, "device", device) != device:
+        raise ValueError(f"the stream is on {stream.device}, the operands on {device}")
     if t.current_device() == index:
         return check(function(*args, t.current_stream(index) if stream is None else stream.cuda_stream))
     with t.device(index):

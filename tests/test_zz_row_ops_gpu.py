@@ -831,3 +831,31 @@ def test_a_call_on_a_stream_that_is_not_the_current_one(pkg, gpu):
     pkg.capi.embedding_lookup(s["table"], s["tokens"], s["h"], scale=2.0, stream=side)
     side.synchronize()
     assert torch.equal(s["h"], want)
+
+
+def test_a_stream_of_another_device_is_refused(pkg, gpu):
+    """The operands would be read by a device that may not reach them.  (The stream below only says so: its address is
+    that of the default stream of the operands' device.)"""
+    torch = _torch()
+    capi = pkg.capi
+
+    class Elsewhere:
+        device = torch.device("cuda", gpu.index + 1)
+        cuda_stream = 0
+
+    f = lambda *s, t=torch.float32: torch.zeros(*s, device=gpu, dtype=t)  # noqa: E731
+    ids, off, plan = f(6, t=torch.int64), f(3, t=torch.int32), capi.RowsPlan(10, 10, 10)
+    calls = [
+        lambda st: capi.embedding_lookup(f(9, 8), ids, f(6, 8), stream=st),
+        lambda st: capi.embedding_grad(plan, ids, f(6, 8), f(9, 8), stream=st),
+        lambda st: capi.group_rows(plan, ids, 4, f(6, t=torch.int32), f(5, t=torch.int32), stream=st),
+        lambda st: capi.grouped_mm(f(6, 8), f(2, 4, 8), off, f(6, 4), stream=st),
+        lambda st: capi.grouped_mm_grad_x(f(6, 4), f(2, 4, 8), off, f(6, 8), stream=st),
+        lambda st: capi.grouped_mm_grad_w(plan, f(6, 4), f(6, 8), off, f(2, 4, 8), stream=st),
+    ]
+    for n, call in enumerate(calls):
+        with pytest.raises(ValueError, match="stream"):
+            call(Elsewhere())
+            pytest.fail(f"call {n} was not refused")
+        call(torch.cuda.current_stream(gpu))
+        call(torch.cuda.ExternalStream(torch.cuda.Stream(gpu).cuda_stream, device=gpu))
