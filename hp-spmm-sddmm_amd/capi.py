@@ -551,7 +551,7 @@ def _weights(t, name, shape, device, dtype):
 def grouped_mm(x, w, offsets, y, stream=None):
     """y[i] = x[i] @ w[e].T for the rows i of every group e through hpspmm_grouped_mm."""
     device = _row_arg(x, "x")
-    (rows, k), (groups, m) = x.shape, w.shape[:2]
+    (rows, k), (groups, m, _) = x.shape, w.shape
     x_p, ld_x, kind = _rows_matrix(x, "x", (rows, k), device)
     w_p, ld_w, stride_w, _ = _weights(w, "w", (groups, m, k), device, x.dtype)
     y_p, ld_y, _ = _rows_matrix(y, "y", (rows, m), device, x.dtype)
@@ -576,7 +576,7 @@ def grouped_mm_grad_w(plan, dy, x, offsets, dw, accumulate=False, stream=None):
     """dw[e] (+)= the sum of dy[i].T @ x[i] over the rows i of group e through hpspmm_grouped_mm_grad_w."""
     handle = _plan_handle(plan)
     device = _row_arg(dy, "dy", plan.device)
-    (rows, m), k, groups = dy.shape, x.shape[1], dw.shape[0]
+    (rows, m), (_, k), (groups, _, _) = dy.shape, x.shape, dw.shape
     dy_p, ld_dy, kind = _rows_matrix(dy, "dy", (rows, m), device)
     x_p, ld_x, _ = _rows_matrix(x, "x", (rows, k), device, dy.dtype)
     dw_p, ld_dw, stride_dw, dw_kind = _weights(dw, "dw", (groups, m, k), device, None)

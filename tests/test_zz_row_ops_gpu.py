@@ -859,3 +859,30 @@ def test_a_stream_of_another_device_is_refused(pkg, gpu):
             pytest.fail(f"call {n} was not refused")
         call(torch.cuda.current_stream(gpu))
         call(torch.cuda.ExternalStream(torch.cuda.Stream(gpu).cuda_stream, device=gpu))
+
+
+def test_operands_of_other_dimensions_are_refused(pkg, gpu):
+    torch = _torch()
+    capi = pkg.capi
+    f = lambda *s, t=torch.float32: torch.zeros(*s, device=gpu, dtype=t)  # noqa: E731
+    ids, off, plan = f(6, t=torch.int64), f(3, t=torch.int32), capi.RowsPlan(10, 10, 10)
+    calls = [
+        lambda: capi.embedding_lookup(f(9), ids, f(6, 8)),
+        lambda: capi.embedding_lookup(f(9, 8), f(6, 1, t=torch.int64), f(6, 8)),
+        lambda: capi.embedding_lookup(f(9, 8), ids, f(6)),
+        lambda: capi.embedding_grad(plan, ids, f(6), f(9, 8)),
+        lambda: capi.embedding_grad(plan, ids, f(6, 8), f(9)),
+        lambda: capi.embedding_grad(plan, f(t=torch.int64), f(6, 8), f(9, 8)),
+        lambda: capi.grouped_mm(f(6), f(2, 4, 8), off, f(6, 4)),
+        lambda: capi.grouped_mm(f(6, 8), f(8), off, f(6, 4)),
+        lambda: capi.grouped_mm(f(6, 8), f(2, 4), off, f(6, 4)),
+        lambda: capi.grouped_mm_grad_x(f(6, 4), f(4, 8), off, f(6, 8)),
+        lambda: capi.grouped_mm_grad_w(plan, f(6), f(6, 8), off, f(2, 4, 8)),
+        lambda: capi.grouped_mm_grad_w(plan, f(6, 4), f(6), off, f(2, 4, 8)),
+        lambda: capi.grouped_mm_grad_w(plan, f(6, 4), f(6, 8), off, f()),
+        lambda: capi.grouped_mm_grad_w(plan, f(6, 4), f(6, 8), off, f(4, 8)),
+    ]
+    for n, call in enumerate(calls):
+        with pytest.raises((TypeError, ValueError)):
+            call()
+            pytest.fail(f"call {n} was not refused")
