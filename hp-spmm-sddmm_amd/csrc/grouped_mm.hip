@@ -54,9 +54,11 @@ int64_t expected_tiles(int mode, const hpspmm::GroupedArgs& g, int64_t edge) {
 // (the rates), 8192 x 8 x 2048 x 2048 113 / 76 / 99, 8192 x 8 x 1024 x 1024 39 / 28 / 30, 2000 x 8 x 1024 x 1024 15 / 13 /
 // 28, 32 x 64 x 2048 x 1024 18 / 24 / 46 (the last two set the rate of 64, which is 580 TFLOP/s in the first); gradient of x
 // of 16384 x 16 x 2048 x 4096, 2.25 rounds of 256, - / 306 / 292.  32-bit
-// products wait for the matrix cores whatever the tile: 1777 x 10 x 1001 x 519, gradient of x 27 / 47 us.
+// products wait for the matrix cores whatever the tile, 64 / 128: 16384 x 16 x 2048 x 2048 1148 / 1102 us (the rate of 64),
+// 8192 x 8 x 1024 x 1024 168 / 193, 20000 x 8 x 512 x 2048 390 / 335, gradient of x of 4096 x 8 x 1024 x 2048 185 / 253, of
+// w 270 / 245, of 1777 x 10 x 1001 x 519 29 / 49.
 int tile_edge(int mode, const hpspmm::GroupedArgs& g, bool wide, bool large) {
-  const struct { int edge; double rate; } kinds[] = {{256, 1030}, {128, 920}, {64, wide ? 800.0 : 490.0}};
+  const struct { int edge; double rate; } kinds[] = {{256, 1030}, {128, 920}, {64, wide ? 885.0 : 490.0}};
   int best = 64;
   double least = 0;
   for (const auto& q : kinds) {

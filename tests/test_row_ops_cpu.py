@@ -119,8 +119,8 @@ def test_python_entry_points_refuse_host_tensors(pkg):
 
 # Sizes (rows, groups, k, m) of grouped products that between them are cut in every way there is; the GPU tests run them.
 TILED = [(300, 5, 129, 65), (1000, 7, 256, 384), (700, 16, 1032, 1032), (9000, 5, 264, 4104), (9000, 5, 4104, 264),
-         (9000, 5, 1028, 2052), (9000, 5, 1001, 1003), (2000, 16, 1016, 1000), (2000, 16, 1001, 1003), (12000, 3, 520, 1032),
-         (9000, 2, 200, 89)]
+         (9000, 5, 1028, 2052), (9000, 5, 1001, 1003), (12000, 3, 1004, 1148), (12000, 3, 1003, 1149), (2000, 16, 1016, 1000),
+         (2000, 16, 1001, 1003), (12000, 3, 520, 1032), (9000, 2, 200, 89)]
 
 
 def tilings(capi, kind, size, case):
