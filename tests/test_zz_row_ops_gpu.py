@@ -886,3 +886,48 @@ def test_operands_of_other_dimensions_are_refused(pkg, gpu):
         with pytest.raises((TypeError, ValueError)):
             call()
             pytest.fail(f"call {n} was not refused")
+
+
+_FIRST_CALLS_CAPTURED = """
+import importlib, sys
+import torch
+sys.path.insert(0, sys.argv[1])
+capi = importlib.import_module("hp-spmm-sddmm_amd").capi
+g = torch.Generator(device="cuda").manual_seed(1)
+whole = lambda *s: torch.randint(-3, 4, s, device="cuda", generator=g).float()
+table, x, w = whole(50, 64), whole(100, 64), whole(3, 32, 64)
+ids = torch.randint(-1, 51, (100,), device="cuda", generator=g)
+offsets = torch.tensor([0, 20, 50, 90], dtype=torch.int32, device="cuda")
+out, y, d_table, dw = (torch.zeros(s, device="cuda") for s in ((100, 64), (100, 32), (50, 64), (3, 32, 64)))
+plan = capi.RowsPlan(100, 50, 64)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    capi.embedding_lookup(table, ids, out, scale=2.0)
+    capi.embedding_grad(plan, ids, x, d_table)
+    capi.grouped_mm(x, w, offsets, y)
+    capi.grouped_mm_grad_w(plan, y, x, offsets, dw)
+for _ in range(3):
+    for t in (out, y, d_table, dw):
+        t.fill_(9.0)
+    graph.replay()
+    torch.cuda.synchronize()
+    here = (ids >= 0) & (ids < 50)
+    assert torch.equal(out, torch.where(here[:, None], 2 * table[ids.clamp(0, 49)], 0.0))
+    assert torch.equal(d_table, torch.zeros_like(d_table).index_add_(0, ids[here], x[here]))
+    assert bool((y[90:] == 9.0).all())
+    for e, (a, b) in enumerate(((0, 20), (20, 50), (50, 90))):
+        assert torch.equal(y[a:b], x[a:b] @ w[e].t())
+        assert torch.equal(dw[e], y[a:b].t() @ x[a:b])
+print("RESULT ok")
+"""
+
+
+def test_first_calls_of_a_process_are_captured(pkg, gpu):
+    """Nothing has run in the process that captures them but the making of a plan (whole numbers: every sum is exact)."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", _FIRST_CALLS_CAPTURED, root], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "RESULT ok" in r.stdout, r.stdout + r.stderr
