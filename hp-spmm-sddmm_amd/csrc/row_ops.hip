@@ -325,14 +325,14 @@ HPSPMM_API int hpspmm_embedding_grad(hpspmm_rows_plan* plan, int64_t n, int64_t 
   // 32768 ids, 131072 x 2048 bf16 161 / 178 us, 262144 ids, 32768 x 1024 f32 208 / 196 us.
   const bool early = !accumulate && n <= vocab && n * width * table_size <= (int64_t)192 << 20;
   const ZeroRows zero = early ? ZeroRows(d_table, vocab, width * table_size, ld_table * table_size) : ZeroRows();
-  Sorted sorted{};
-  if (int rc = sort_rows(plan, n, vocab, d_ids, id_type, nullptr, nullptr, zero, st, &sorted)) return rc;
   const SumShape s = sum_shape(n, width, 16 / grad_size);
   if (2 * s.chunks * s.pitch > plan->carry_floats) return fail(HPSPMM_ERR_INVALID_ARG, "the plan's workspace is too small");
   const int64_t per_block = s.tpr_log2 < 6 ? hpspmm::kBlock >> s.tpr_log2 : 1;
   const int64_t sum_blocks = ceil_div(s.chunks, per_block);
   const int64_t zero_blocks = accumulate || early ? 0 : std::min<int64_t>(ceil_div(vocab, hpspmm::kZeroRows), 1 << 20);
   const unsigned threads = s.tpr_log2 < 6 ? hpspmm::kBlock : 1u << s.tpr_log2;
+  Sorted sorted{};
+  if (int rc = sort_rows(plan, n, vocab, d_ids, id_type, nullptr, nullptr, zero, st, &sorted)) return rc;
   const bool whole = aligned_to(d_grad, 16) && aligned_to(d_table, 16) && ld_grad * grad_size % 16 == 0 &&
                      ld_table * table_size % 16 == 0 && width * grad_size % 16 == 0;
   const hpspmm::SumArgs g{n, (uint32_t)vocab, (int32_t)width, (int32_t)s.pitch, sorted.keys, sorted.rows, d_grad, ld_grad, scale,
