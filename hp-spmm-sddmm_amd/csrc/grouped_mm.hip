@@ -7,7 +7,8 @@ using namespace hpspmm_host;
 
 namespace {
 
-// Groups are a grid dimension of the gradient of the weights.
+// Every workgroup of a product finds its tile's group by a walk over all offsets: 4096 groups of 64 x 64 (4096 rows) take 116
+// us, 65535 of them (131072 rows) 34 ms, nearly all of it the search.  More groups than that are refused.
 constexpr int64_t kMaxGroups = 65535;
 
 int check_grouped(int64_t rows, int64_t groups, int64_t k, int64_t m, const int32_t* d_offsets, int dtype) {
@@ -50,10 +51,11 @@ int64_t expected_tiles(int mode, const hpspmm::GroupedArgs& g, int64_t edge) {
 
 // Edge of the output tiles, 256 (16-bit operands at multiples of 16 bytes), 128 or 64: the one that is expected to take
 // the least time, tiles per CU (one at least, and a part of a round that is not full) times the area of a tile over its
-// rate.  bf16, rows x groups x k x m, product with tiles of 64 / 128 / 256 in us: 32768 x 32 x 2048 x 4096 933 / 588 / 526
-// (the rates), 8192 x 8 x 2048 x 2048 113 / 76 / 99, 8192 x 8 x 1024 x 1024 39 / 28 / 30, 2000 x 8 x 1024 x 1024 15 / 13 /
-// 28, 32 x 64 x 2048 x 1024 18 / 24 / 46 (the last two set the rate of 64, which is 580 TFLOP/s in the first); gradient of x
-// of 16384 x 16 x 2048 x 4096, 2.25 rounds of 256, - / 306 / 292.  32-bit
+// rate.  bf16, rows x groups x k x m, product with tiles of 64 / 128 / 256, us a call among many on three sets of operands in
+// turn: 32768 x 32 x 2048 x 4096 980 / 622 / 544, 8192 x 8 x 2048 x 2048 132 / 89 / 103, 8192 x 8 x 1024 x 1024 44 / 30 / 30,
+// 2000 x 8 x 1024 x 1024 18 / 14 / 29, 32 x 64 x 2048 x 1024 22 / 31 / 49; gradient of x of 16384 x 16 x 2048 x 4096, 2.25
+// rounds of 256, - / 322 / 304.  Only the ratios of the rates count: 128 to 256 is the first line's 0.875 raised to 0.893, from
+// 0.888 on the second line gets its 128; 64 to 128 is set by the last two (the first line alone would have it 0.63).  32-bit
 // products wait for the matrix cores whatever the tile, 64 / 128: 16384 x 16 x 2048 x 2048 1148 / 1102 us (the rate of 64),
 // 8192 x 8 x 1024 x 1024 168 / 193, 20000 x 8 x 512 x 2048 390 / 335, gradient of x of 4096 x 8 x 1024 x 2048 185 / 253, of
 // w 270 / 245, of 1777 x 10 x 1001 x 519 29 / 49.
@@ -88,7 +90,7 @@ int launch_tiles(const hpspmm::GroupedArgs& g, hipStream_t st) {
 
 // Parts that the rows of every group are cut into for the gradient of the weights, 1 = none: where there are few output
 // tiles and long groups, as many as give every slot of the chip a tile, each of at least 4 steps of the mean group.
-// 18867 x 2 x 2304 x 89 bf16 131 -> 41 us, 32768 x 1 x 512 x 512 131 -> 30 us, 9000 x 2 x 200 x 89 34 -> 18 us.
+// 18867 x 2 x 2304 x 89 bf16 116 -> 42 us, 32768 x 1 x 512 x 512 130 -> 31 us, 9000 x 2 x 200 x 89 51 -> 18 us.
 int row_splits(const hpspmm::GroupedArgs& g, int64_t depth) {
   const int64_t tiles = expected_tiles(hpspmm::kGradW, g, hpspmm::kSplitEdge);
   const int64_t steps = g.rows / g.groups / depth;

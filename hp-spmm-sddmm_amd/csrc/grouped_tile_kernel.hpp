@@ -14,11 +14,13 @@
 // terms beyond the contraction are zeros in both operands, whatever lies there in memory.
 //
 // Sums are held in 32 bits by the matrix instructions (16 x 16 x 32 for 16-bit, 16 x 16 x 4 for 32-bit elements) and
-// rounded once.  bf16, 32768 rows, 32 groups, k 2048, m 4096, tiles of 256: product 526 us (1029 TFLOP/s), gradient of x
-// 522 us, of w in 32 bits 699 us; the matrix cores are busy 55, 58 and 44 % of the time, an eighth of it with rows beyond
-// the ends of groups.  What bounds it is the way of the operands into LDS: without the products the same loads take 510 us,
-// without the loads the products 405 us; a CU has about 64 lines under way, at 570 cycles each (a larger tile, fewer
-// bytes, does not fit 160 KB of LDS).  Reads of LDS meet no bank conflicts in any of the three.  On the way: loads with
+// rounded once.  bf16, 32768 rows, 32 groups, k 2048, m 4096, tiles of 256, a call among many on three sets of operands in
+// turn: product 544 us (995 TFLOP/s), gradient of x 543 us, of w in 32 bits 736 us; 16384 rows, 16 groups: 292, 304 and 374.
+// The matrix cores are busy 55 % of the product's time (of the gradients' at 16384 rows 46 and 41 %), an eighth of it with
+// rows beyond the ends of groups.  What bounds it is the way of the operands into LDS: without the products the same loads
+// take 510 us, without the loads the products 405 us (one set of operands again and again); a CU has about 64 lines under
+// way, at 570 cycles each (a larger tile, fewer bytes, does not fit 160 KB of LDS).  The steps' reads of LDS meet no bank
+// conflicts in any of the three.  On the way, likewise on one set: loads with
 // the builtin, whose counter every transposed read waits for, 715 / 944 us for the gradients; steps of 32 terms, half a
 // line a row, 650 / 870 / 1155 us; tiles in rows instead of panels, a third more requests to memory, 575 instead of 562 us.
 #pragma once
@@ -451,7 +453,8 @@ __global__ __launch_bounds__(64 * kWM * kWN, 2) void grouped_tile_kernel(Grouped
           }
         }
         // Gradients of large weights go past the caches, which they do not fit: 16 matrices of 4096 x 2048 in 32 bits from
-        // 16384 rows 425 -> 343 us, of 4096 x 4096 868 -> 688 us; products and gradients of x gain nothing by it.
+        // 16384 rows 389 -> 374 us (402 -> 355 where the same operands come again and stay in the caches), of 4096 x 4096
+        // 768 -> 733 us (798 -> 704); products and gradients of x gain nothing by it.
         if constexpr (kMode == kGradW && kBM == 256) __builtin_nontemporal_store(v, reinterpret_cast<Loose*>(at));
         else *reinterpret_cast<Loose*>(at) = v;
       } else {

@@ -9,9 +9,9 @@ namespace hpspmm {
 // out[i, :] = scale * table[ids[i], :], rows of zeros for ids outside the table: one product in 32 bits, rounded once.
 // Bound by the bytes, n rows read and n written.  A thread owns 16 bytes of a row; 2^tpr_log2 adjacent threads share a
 // row's column tile, a workgroup covers kRows rows one after the other, all of whose loads are in flight together.
-// kStream: large outputs go past the caches, which they do not fit (32768 rows of 4096 bf16 over 131072: 84 -> 63 us with
-// the table's rows partly in the caches; 82 us = 4.5 TB/s of distinct rows and output where they are not).  16 rows of
-// 1024 take 7 us from Python, half of it the launch.
+// kStream: large outputs go past the caches, which they do not fit (32768 rows of 4096 bf16 over 131072, 12651 different
+// ones: 87 -> 81 us, 4.6 TB/s of different rows and output; 85 -> 63 us where the same rows come again and stay in the
+// caches).  16 rows of 1024 take 7 us from Python, half of it the launch.
 template <class T, class Id, bool kAligned, int kRows, bool kStream>
 __global__ __launch_bounds__(kBlock) void embedding_lookup_kernel(int64_t n, uint32_t vocab, int32_t width, int tpr_log2,
                                                                  const Id* __restrict__ ids, const T* __restrict__ table,

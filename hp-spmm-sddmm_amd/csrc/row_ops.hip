@@ -321,18 +321,22 @@ HPSPMM_API int hpspmm_embedding_grad(hpspmm_rows_plan* plan, int64_t n, int64_t 
   const int64_t grad_size = dtype_size(grad_type), table_size = dtype_size(table_type);
   // Rows that no id points at become zeros either in the launches of the sort, which leave most of the chip idle but know
   // of no row yet (so every row is filled), or beside the sums, where the rows that get one are left out.  The first hides
-  // the sort behind the fill and writes the rows that get a sum twice.  Early / late: 1000 ids, 50001 x 771 f32 28 / 36 us,
-  // 32768 ids, 131072 x 2048 bf16 161 / 178 us, 262144 ids, 32768 x 1024 f32 208 / 196 us.
+  // the sort behind the fill and writes the rows that get a sum twice.  Early / late, 2048 columns bf16 -> bf16, as many ids
+  // as rows of the table, frequencies of natural text or even ones: 64 MB of rows 58 / 65 or 59 / 62 us, 128 MB 97 / 99 or
+  // 104 / 98, 192 MB 136 / 138 or 143 / 132, 256 MB 170 / 170 or 177 / 160, 512 MB 285 / 274 or 312 / 270, 1 GB 531 / 495 or
+  // 603 / 505; a fourth as many ids as rows of the table: 64 MB 89 / 110 or 89 / 105, 128 MB 165 / 180 or 171 / 176, 192 MB
+  // 239 / 252 or 249 / 245, 256 MB 307 / 310 or 320 / 302, 512 MB 582 / 554 or 624 / 561.  (1000 ids, 50001 x 771 f32 28 / 36;
+  // more ids than rows, 262144 over 32768 x 1024 f32: 208 / 196.)
   const bool early = !accumulate && n <= vocab && n * width * table_size <= (int64_t)192 << 20;
   const ZeroRows zero = early ? ZeroRows(d_table, vocab, width * table_size, ld_table * table_size) : ZeroRows();
   const SumShape s = sum_shape(n, width, 16 / grad_size);
   if (2 * s.chunks * s.pitch > plan->carry_floats) return fail(HPSPMM_ERR_INVALID_ARG, "the plan's workspace is too small");
+  Sorted sorted{};
+  if (int rc = sort_rows(plan, n, vocab, d_ids, id_type, nullptr, nullptr, zero, st, &sorted)) return rc;
   const int64_t per_block = s.tpr_log2 < 6 ? hpspmm::kBlock >> s.tpr_log2 : 1;
   const int64_t sum_blocks = ceil_div(s.chunks, per_block);
   const int64_t zero_blocks = accumulate || early ? 0 : std::min<int64_t>(ceil_div(vocab, hpspmm::kZeroRows), 1 << 20);
   const unsigned threads = s.tpr_log2 < 6 ? hpspmm::kBlock : 1u << s.tpr_log2;
-  Sorted sorted{};
-  if (int rc = sort_rows(plan, n, vocab, d_ids, id_type, nullptr, nullptr, zero, st, &sorted)) return rc;
   const bool whole = aligned_to(d_grad, 16) && aligned_to(d_table, 16) && ld_grad * grad_size % 16 == 0 &&
                      ld_table * table_size % 16 == 0 && width * grad_size % 16 == 0;
   const hpspmm::SumArgs g{n, (uint32_t)vocab, (int32_t)width, (int32_t)s.pitch, sorted.keys, sorted.rows, d_grad, ld_grad, scale,

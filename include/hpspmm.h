@@ -486,7 +486,10 @@ int hpspmm_group_rows(hpspmm_rows_plan *plan, int64_t n, int64_t groups, const v
  * stride_w elements apart).  offsets holds groups + 1 entries on the device,
  * not decreasing, within [0, rows]; rows of no group are not read and stay as
  * they are in the output.  (Offsets that are otherwise give unspecified values,
- * never an access out of range.)  groups <= 65535; k, m <= 2^20.
+ * never an access out of range.)  groups <= 65535 (every workgroup looks through
+ * the offsets: made for up to some hundreds of groups); k, m <= 2^20; a product
+ * of more than 2^22 - 8 output tiles of 256 x 256 or 2^23 - 8 smaller ones
+ * (hpspmm_grouped_tiling) is refused.
  *
  *   hpspmm_grouped_mm           y[i, :]  = x[i, :] * w[e]^T     y is rows x m
  *   hpspmm_grouped_mm_grad_x    dx[i, :] = dy[i, :] * w[e]      dx is rows x k
