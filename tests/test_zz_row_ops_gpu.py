@@ -931,3 +931,144 @@ def test_first_calls_of_a_process_are_captured(pkg, gpu):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", _FIRST_CALLS_CAPTURED, root], capture_output=True, text=True, timeout=100)
     assert r.returncode == 0 and "RESULT ok" in r.stdout, r.stdout + r.stderr
+
+
+# ---- the far ends of what may be asked for --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float32"])
+@pytest.mark.parametrize("rows, groups, k, m", [(70, 2, 1 << 20, 40), (70, 2, 40, 1 << 20), (70, 2, (1 << 20) - 1, 9)])
+def test_grouped_products_of_the_longest_rows(pkg, gpu, kind, rows, groups, k, m):
+    test_grouped_products(pkg, gpu, kind, "contiguous", "even", rows, groups, k, m)
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float32"])
+def test_grouped_products_of_rows_far_apart(pkg, gpu, kind):
+    """Rows 2^21 + 8 elements apart: more than the offsets of the direct loads hold."""
+    torch = _torch()
+    capi = pkg.capi
+    g = _gen(gpu, 21)
+    rows, groups, k, m, ld = 300, 3, 72, 40, (1 << 21) + 8
+
+    def apart(n, width):
+        t = torch.empty(n, ld, device=gpu, dtype=_t(kind))[:, :width]
+        t.copy_(torch.randn(n, width, device=gpu, generator=g))
+        return t
+
+    x, dy, w = apart(rows, k), apart(rows, m), torch.stack([torch.randn(m, k, device=gpu, generator=g).to(_t(kind))] * groups)
+    offsets = torch.tensor([0, 70, 200, 300], dtype=torch.int32, device=gpu)
+    near = [t.contiguous() for t in (x, dy)]
+    wide = apart(groups * m, k).unflatten(0, (groups, m))
+    wide.copy_(w)
+    far = (capi.grouped_mm(x, wide, offsets, apart(rows, m)), capi.grouped_mm_grad_x(dy, wide, offsets, apart(rows, k)),
+           capi.grouped_mm_grad_w(capi.RowsPlan(0, 0), dy, x, offsets, apart(groups * m, k).unflatten(0, (groups, m))))
+    for e in range(groups):
+        r = slice(int(offsets[e]), int(offsets[e + 1]))
+        xe, de, we = near[0][r].double(), near[1][r].double(), w[e].double()
+        _check(far[0][r].contiguous(), xe @ we.t().contiguous(), xe.abs() @ we.abs().t().contiguous(), k)
+        _check(far[1][r].contiguous(), de @ we, de.abs() @ we.abs(), m)
+        _check(far[2][e].contiguous(), de.t().contiguous() @ xe, de.abs().t().contiguous() @ xe.abs(), r.stop - r.start)
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float32"])
+@pytest.mark.parametrize("width", [1 << 20, (1 << 20) - 3])
+def test_lookup_and_gradient_of_the_longest_rows(pkg, gpu, kind, width):
+    test_lookup(pkg, gpu, kind, "int32", "contiguous", 45, 9, width)
+    test_lookup_gradient(pkg, gpu, kind, "same", "contiguous", "mixed", 45, 9, width)
+
+
+@pytest.mark.parametrize("k, m", [(4104, 72), (72, 4104), (4101, 67)])
+def test_grouped_products_beyond_32_bit_offsets(pkg, gpu, k, m):
+    """Rows or outputs of more than 2^32 bytes and 2^31 elements: what lies at both ends, and the sums over all of it."""
+    torch = _torch()
+    capi = pkg.capi
+    g = _gen(gpu, k)
+    rows = (1 << 19) + 4001
+    x = torch.zeros(rows, k, device=gpu, dtype=torch.bfloat16)
+    dy = torch.zeros(rows, m, device=gpu, dtype=torch.bfloat16)
+    ends = torch.cat([torch.arange(40, device=gpu), torch.arange(rows - 300, rows, device=gpu)])
+    x[ends] = torch.randn(ends.numel(), k, device=gpu, generator=g).bfloat16()
+    dy[ends] = torch.randn(ends.numel(), m, device=gpu, generator=g).bfloat16()
+    w = torch.randn(3, m, k, device=gpu, generator=g).bfloat16()
+    bounds = [0, 30, rows - 100, rows]
+    offsets = torch.tensor(bounds, dtype=torch.int32, device=gpu)
+    y = capi.grouped_mm(x, w, offsets, torch.empty_like(dy))
+    dx = capi.grouped_mm_grad_x(dy, w, offsets, torch.empty_like(x))
+    dw = capi.grouped_mm_grad_w(capi.RowsPlan(0, 0), dy, x, offsets, torch.empty(3, m, k, device=gpu))
+    for e in range(3):
+        at = ends[(ends >= bounds[e]) & (ends < bounds[e + 1])]
+        xe, de, we = x[at].double(), dy[at].double(), w[e].double()
+        _check(y[at], xe @ we.t().contiguous(), xe.abs() @ we.abs().t().contiguous(), k)
+        _check(dx[at], de @ we, de.abs() @ we.abs(), m)
+        _check(dw[e], de.t().contiguous() @ xe, de.abs().t().contiguous() @ xe.abs(), bounds[e + 1] - bounds[e])
+    assert not y[40:rows - 300].any() and not dx[40:rows - 300].any()
+
+
+def test_grouped_weights_beyond_32_bit_offsets(pkg, gpu):
+    torch = _torch()
+    capi = pkg.capi
+    g = _gen(gpu, 23)
+    rows, groups, k, m = 400, 130, 4104, 4112
+    x, dy = torch.randn(rows, k, device=gpu, generator=g).bfloat16(), torch.randn(rows, m, device=gpu, generator=g).bfloat16()
+    w = torch.empty(groups, m, k, device=gpu, dtype=torch.bfloat16).normal_(generator=g)
+    assert w.numel() > 1 << 31
+    off = np.concatenate([[0], np.cumsum([150] + [0] * (groups - 3) + [100, 140])])
+    offsets = torch.from_numpy(off.astype(np.int32)).to(gpu)
+    y = capi.grouped_mm(x, w, offsets, torch.empty_like(dy))
+    dx = capi.grouped_mm_grad_x(dy, w, offsets, torch.empty_like(x))
+    dw = capi.grouped_mm_grad_w(capi.RowsPlan(0, 0), dy, x, offsets, torch.empty_like(w))
+    for e in (0, groups - 2, groups - 1):
+        r = slice(int(off[e]), int(off[e + 1]))
+        xe, de, we = x[r].double(), dy[r].double(), w[e].double()
+        _check(y[r], xe @ we.t().contiguous(), xe.abs() @ we.abs().t().contiguous(), k)
+        _check(dx[r], de @ we, de.abs() @ we.abs(), m)
+        _check(dw[e], de.t().contiguous() @ xe, de.abs().t().contiguous() @ xe.abs(), r.stop - r.start)
+    assert not dw[1:groups - 2].any()
+
+
+def test_lookup_gradient_beyond_32_bit_offsets(pkg, gpu):
+    """Rows and a table of more than 2^32 bytes and 2^31 elements, with what is not zero at their far ends."""
+    torch = _torch()
+    n = vocab = (1 << 19) + 77
+    width = 4100
+    g = _gen(gpu, 24)
+    grad = torch.zeros(n, width, device=gpu, dtype=torch.bfloat16)
+    ends = torch.tensor([0, 1, 5, n - 9, n - 2, n - 1], device=gpu)
+    grad[ends] = torch.randn(6, width, device=gpu, generator=g).bfloat16()
+    ids = torch.arange(n, device=gpu).flip(0).contiguous()
+    ids[n - 2] = ids[5] = vocab - 3
+    d_table = torch.full((vocab, width), float("nan"), device=gpu, dtype=torch.bfloat16)
+    pkg.capi.embedding_grad(pkg.capi.RowsPlan(n, vocab, width), ids, grad, d_table)
+    value, absolute, count = _grad_reference(ids[ends], grad[ends], vocab, 1.0)
+    met = ids[ends].unique()
+    _check(d_table[met], value[met], absolute[met], count[met])
+    d_table[met] = 0.0
+    for r in range(0, vocab, 1 << 16):
+        assert not d_table[r:r + (1 << 16)].any() and not torch_isnan(d_table[r:r + (1 << 16)])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("layout", ["contiguous", "odd_slice"])
+@pytest.mark.parametrize("rows, groups, k, m", [(300, 5, 136, 72), (9000, 2, 200, 88), (2000, 16, 1016, 1000), (9000, 5, 264, 1032)])
+def test_grouped_gradients_keep_nan_and_inf_in_their_groups(pkg, gpu, kind, layout, rows, groups, k, m):
+    """The largest group's rows and weights are NaN or infinite: every other group's results have the bits that they have with
+    ordinary values there."""
+    torch = _torch()
+    capi = pkg.capi
+    x, dy, w, off, offsets, free = _experts(gpu, rows, rows, groups, k, m, kind, layout, "ragged")
+    odd = int(np.argmax(np.diff(off)))
+    rest = [e for e in range(groups) if e != odd]
+    other = torch.ones(rows, dtype=torch.bool, device=gpu) & ~free
+    other[int(off[odd]):int(off[odd + 1])] = False
+    plan, got = capi.RowsPlan(0, 0), []
+    for fill in (1.0, float("nan"), float("inf")):
+        for t in (x, dy):
+            t[int(off[odd]):int(off[odd + 1])] = fill
+        w[odd] = fill
+        y, dx = torch.zeros(rows, m, device=gpu, dtype=_t(kind)), torch.zeros(rows, k, device=gpu, dtype=_t(kind))
+        dw = torch.zeros(groups, m, k, device=gpu, dtype=_t(kind))
+        capi.grouped_mm(x, w, offsets, y), capi.grouped_mm_grad_x(dy, w, offsets, dx), capi.grouped_mm_grad_w(plan, dy, x, offsets, dw)
+        got.append((y[other], dx[other], dw[rest]))
+    assert off[odd + 1] > off[odd]
+    for q in range(3):
+        assert bool(torch.isfinite(got[0][q]).all())
+        assert torch.equal(got[0][q], got[1][q]) and torch.equal(got[0][q], got[2][q]), q
